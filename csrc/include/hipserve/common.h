@@ -276,4 +276,30 @@ HS_DEVICE void sum_slices8(f32x4& lo, f32x4& hi, const float* __restrict__ p, lo
   }
 }
 
+// sum over S slices of 8 consecutive fp32 partials, rounded to bf16 like the unfused reduce output, returned as fp32
+HS_DEVICE void sum8_bf16(float (&o)[8], const float* __restrict__ p, long slice, int S) {
+  f32x4 lo, hi;
+  sum_slices8(lo, hi, p, slice, S);
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    o[j] = bf16_to_f32(f32_to_bf16(lo[j]));
+    o[j + 4] = bf16_to_f32(f32_to_bf16(hi[j]));
+  }
+}
+
+// x = bf16(x + b) for 8 bf16 bias values (torch's bf16 add of the bias vector)
+HS_DEVICE void add_bias8(float (&x)[8], const unsigned short* __restrict__ b) {
+  const u16x8 v = *reinterpret_cast<const u16x8*>(b);
+#pragma unroll
+  for (int j = 0; j < 8; ++j) x[j] = bf16_to_f32(f32_to_bf16(x[j] + bf16_to_f32(v[j])));
+}
+
+// out16 (optional): an f16 copy of the bf16 output in the quantised decode GEMMs' staging
+// pair order {0, 2, 1, 3, 4, 6, 5, 7} per aligned 8-run — the o-projection's x16 operand
+// (gguf_mfma.hip), written here instead of by a conversion kernel
+HS_DEVICE void store_o16(unsigned short* __restrict__ out16, long row_off, int e, unsigned short bf) {
+  const int p = (e & ~7) | (e & 4) | ((e & 1) << 1) | ((e >> 1) & 1);
+  out16[row_off + p] = __builtin_bit_cast(unsigned short, static_cast<_Float16>(bf16_to_f32(bf)));
+}
+
 }  // namespace hipserve

@@ -58,6 +58,39 @@ void launch_prefill_attention(void* out, long out_stride, const void* q,
                               const int* tiles, int ntiles, int nq, int nkv, int D,
                               int block_size, float scale, int window, hipStream_t s, bool kv_f8 = false);
 
+// kv4_cache.hip, kv4_decode.hip, kv4_prefill.hip — the 4-bit paged KV cache (layout: kv4.h)
+struct Kv4Cache {
+  void* k;
+  void* v;
+  long blocks;
+  int nkv, D, block_size;
+};
+// a step's queries rotated in place (or, from the partials, into qkv), its keys and values into the cache. ws: the qkv
+// projection's split-K partials [S, T, (nq + 2 nkv) D] with the options of launch_splitk_rope_cache, or null: the rows of qkv.
+// A slot outside of the cache writes nothing.
+void launch_kv4_write(void* qkv, long qkv_stride, const float* ws, int S, const void* bias, const float* qw,
+                      const float* kw, float eps, const long* positions, const long* slots, const float* cos_sin,
+                      long max_pos, const Kv4Cache& c, int T, int nq, int mode, hipStream_t s);
+// rows of slots as bf16 [T, nkv, D]; zeros for a slot outside of the cache
+void launch_kv4_read(void* k_out, long k_stride, void* v_out, long v_stride, const Kv4Cache& c, const long* slots, int T,
+                     hipStream_t s);
+struct Kv4Attn {
+  void* out;
+  long out_stride;
+  const void* q;
+  long q_stride;
+  Kv4Cache cache;
+  const int* block_tables;
+  int bt_stride, bt_width;
+  int nq;
+  float scale;
+  int window, sinks;  // window > 0: keys within window - 1 positions before the query, and the first `sinks` ones
+};
+void launch_kv4_decode(const Kv4Attn& a, const int* context_lens, float* tmp_out, float* tmp_ml, int B, int part_size,
+                       int max_parts, void* out16, hipStream_t s);
+void launch_kv4_prefill(const Kv4Attn& a, const int* cu_q, int seqs, const int* ctx_lens, int rows, const int* tiles,
+                        int ntiles, hipStream_t s);
+
 // sampling.hip
 // ws: fp32 workspace of sample_workspace_floats(rows, V) for the multi-CU path
 // (vocab >= 8192); nullptr selects the one-workgroup-per-row kernel.

@@ -17,15 +17,6 @@
 
 namespace hipserve {
 
-// sum over S slices of 8 consecutive fp32 partials (batched loads, common.h),
-// rounded to bf16 like the unfused reduce output, returned as fp32
-// x = bf16(x + b) for 8 bf16 bias values (torch's bf16 add of the bias vector)
-HS_DEVICE void add_bias8(float (&x)[8], const unsigned short* __restrict__ b) {
-  const u16x8 v = *reinterpret_cast<const u16x8*>(b);
-#pragma unroll
-  for (int j = 0; j < 8; ++j) x[j] = bf16_to_f32(f32_to_bf16(x[j] + bf16_to_f32(v[j])));
-}
-
 // 8 bf16 values -> f16 in the quantised decode GEMM's staging pair order
 // {0, 2, 1, 3, 4, 6, 5, 7} (gguf_mfma.hip kX16): bf16 -> fp32 exact, -> f16 round to
 // nearest — the conversion the GEMM would otherwise run in every workgroup
@@ -35,16 +26,6 @@ HS_DEVICE u16x8 f16_pairs8(const u16x8 v) {
 #pragma unroll
   for (int j = 0; j < 8; ++j) h[j] = __builtin_bit_cast(unsigned short, static_cast<_Float16>(bf16_to_f32(v[ord[j]])));
   return h;
-}
-
-HS_DEVICE void sum8_bf16(float (&o)[8], const float* __restrict__ p, long slice, int S) {
-  f32x4 lo, hi;
-  sum_slices8(lo, hi, p, slice, S);
-#pragma unroll
-  for (int j = 0; j < 4; ++j) {
-    o[j] = bf16_to_f32(f32_to_bf16(lo[j]));
-    o[j + 4] = bf16_to_f32(f32_to_bf16(hi[j]));
-  }
 }
 
 template <int NT, int VPT, bool kWF32>

@@ -237,6 +237,161 @@ void prefill_attention(at::Tensor& out, const at::Tensor& q, const at::Tensor& k
                                      (float)scale, (int)window, cur_stream(), kv_is_f8(k_cache, v_cache));
 }
 
+// ---- the 4-bit paged KV cache (--kv-cache-dtype mxfp4): uint8 [blocks, nkv, block_size, 17 head_dim / 32], K and V alike
+static hipserve::Kv4Cache kv4_cache(const at::Tensor& k, const at::Tensor& v, int64_t nkv, const char* who) {
+  TORCH_CHECK(k.scalar_type() == at::kByte && v.scalar_type() == at::kByte && k.dim() == 4 && k.sizes() == v.sizes() &&
+                  k.is_contiguous() && v.is_contiguous() && k.is_cuda() && v.device() == k.device(),
+              who, ": mxfp4 caches are contiguous uint8 [blocks, kv heads, block_size, 17 head_dim / 32], K and V alike");
+  TORCH_CHECK(nkv > 0 && k.size(1) == nkv, who, ": the cache has ", k.size(1), " kv heads, not ", nkv);
+  const int64_t w = k.size(3), bs = k.size(2), D = w * 32 / 17;
+  TORCH_CHECK(w % 17 == 0 && (D == 64 || D == 96 || D == 128), who, ": head_dim 64, 96 or 128");
+  TORCH_CHECK(bs >= 16 && bs <= 256 && (bs & (bs - 1)) == 0, who, ": block_size a power of two in [16, 256]");
+  TORCH_CHECK(k.size(0) > 0 && k.size(0) <= INT32_MAX, who, ": the cache has no blocks, or more than a block table can name");
+  return {k.data_ptr(), v.data_ptr(), k.size(0), (int)nkv, (int)D, (int)bs};
+}
+// rows of bf16 that the kernels take 16 bytes at a time
+static void kv4_rows(const at::Tensor& x, const at::Tensor& cache, int64_t cols, const char* who, const char* name) {
+  TORCH_CHECK(x.device() == cache.device() && x.scalar_type() == at::kBFloat16 && x.dim() == 2 && x.size(1) >= cols &&
+                  (x.size(0) <= 1 || x.stride(0) >= cols) && x.stride(1) == 1,
+              who, ": ", name, " are bf16 rows of at least ", cols, " on the cache's device");
+  TORCH_CHECK(x.stride(0) % 8 == 0 && reinterpret_cast<uintptr_t>(x.data_ptr()) % 16 == 0, who, ": ", name,
+              " start at multiples of 16 bytes");
+  TORCH_CHECK(x.size(0) < (1LL << 30), who, ": too many rows");
+}
+static const int64_t* kv4_longs(const at::Tensor& x, const at::Tensor& cache, int64_t n, const char* who, const char* name) {
+  TORCH_CHECK(x.device() == cache.device() && x.scalar_type() == at::kLong && x.is_contiguous() && x.numel() >= n, who, ": ",
+              name, " are contiguous int64, one a row");
+  return x.data_ptr<int64_t>();
+}
+static const int* kv4_ints(const at::Tensor& x, const at::Tensor& cache, int64_t n, const char* who, const char* name) {
+  TORCH_CHECK(x.device() == cache.device() && x.scalar_type() == at::kInt && x.is_contiguous() && x.numel() >= n, who, ": ",
+              name, " are contiguous int32, at least ", n);
+  return x.data_ptr<int>();
+}
+static void kv4_write(at::Tensor& qkv, const at::Tensor* ws, int64_t splits, const at::Tensor& positions,
+                      const at::Tensor& slots, const at::Tensor& cos_sin, at::Tensor& k_cache, at::Tensor& v_cache,
+                      int64_t nq, int64_t nkv, int64_t head_dim, int64_t mode, const at::Tensor* bias,
+                      const at::Tensor* q_w, const at::Tensor* k_w, double eps, const char* who) {
+  const hipserve::Kv4Cache c = kv4_cache(k_cache, v_cache, nkv, who);
+  TORCH_CHECK(c.D == head_dim, who, ": the cache holds heads of ", c.D);
+  TORCH_CHECK(nq >= 0 && (mode == 0 || mode == 1), who, ": nq >= 0, mode 0 (rotate-half) or 1 (neighbouring dims)");
+  const int64_t T = qkv.size(0), N = (nq + 2 * nkv) * head_dim;
+  kv4_rows(qkv, k_cache, N, who, "qkv");
+  const int64_t* pos = kv4_longs(positions, k_cache, T, who, "positions");
+  const int64_t* sl = kv4_longs(slots, k_cache, T, who, "slots");
+  TORCH_CHECK(cos_sin.device() == k_cache.device() && cos_sin.scalar_type() == at::kFloat && cos_sin.dim() == 2 &&
+                  cos_sin.size(0) > 0 && cos_sin.size(1) == head_dim && cos_sin.is_contiguous(),
+              who, ": cos_sin fp32 [positions, head_dim]");
+  if (ws != nullptr)
+    TORCH_CHECK(ws->device() == k_cache.device() && ws->scalar_type() == at::kFloat && ws->is_contiguous() && splits > 0 &&
+                    ws->numel() >= splits * T * N,
+                who, ": fp32 partials [splits, rows, (nq + 2 nkv) head_dim]");
+  if (bias != nullptr)
+    TORCH_CHECK(bias->device() == k_cache.device() && bias->scalar_type() == at::kBFloat16 && bias->is_contiguous() &&
+                    bias->numel() == N && reinterpret_cast<uintptr_t>(bias->data_ptr()) % 16 == 0,
+                who, ": bias bf16 [(nq + 2 nkv) head_dim]");
+  TORCH_CHECK((q_w == nullptr) == (k_w == nullptr), who, ": q and k norm weights come together");
+  if (q_w != nullptr) {
+    for (const at::Tensor* w : {q_w, k_w})
+      TORCH_CHECK(w->device() == k_cache.device() && w->scalar_type() == at::kFloat && w->is_contiguous() &&
+                      w->numel() == head_dim,
+                  who, ": q / k norm weights fp32 [head_dim]");
+    TORCH_CHECK(mode == 0 && head_dim != 96, who, ": q / k norm needs mode 0 and head_dim 64 or 128");
+  }
+  c10::hip::HIPGuardMasqueradingAsCUDA g(k_cache.device());
+  hipserve::launch_kv4_write(qkv.data_ptr(), qkv.stride(0), ws ? ws->data_ptr<float>() : nullptr, (int)splits,
+                             bias ? bias->data_ptr() : nullptr, q_w ? q_w->data_ptr<float>() : nullptr,
+                             k_w ? k_w->data_ptr<float>() : nullptr, (float)eps, pos, sl, cos_sin.data_ptr<float>(),
+                             cos_sin.size(0), c, (int)T, (int)nq, (int)mode, cur_stream());
+}
+void rope_cache_mx4(at::Tensor& qkv, const at::Tensor& positions, const at::Tensor& slots, const at::Tensor& cos_sin,
+                    at::Tensor& k_cache, at::Tensor& v_cache, int64_t nq, int64_t nkv, int64_t head_dim, int64_t mode) {
+  kv4_write(qkv, nullptr, 0, positions, slots, cos_sin, k_cache, v_cache, nq, nkv, head_dim, mode, nullptr, nullptr, nullptr,
+            0.0, "rope_cache");
+}
+void splitk_rope_cache_mx4(at::Tensor& qkv, const at::Tensor& ws, int64_t splits, const at::Tensor& positions,
+                           const at::Tensor& slots, const at::Tensor& cos_sin, at::Tensor& k_cache, at::Tensor& v_cache,
+                           int64_t nq, int64_t nkv, int64_t head_dim, int64_t mode, const c10::optional<at::Tensor>& bias,
+                           const c10::optional<at::Tensor>& q_w, const c10::optional<at::Tensor>& k_w, double eps) {
+  kv4_write(qkv, &ws, splits, positions, slots, cos_sin, k_cache, v_cache, nq, nkv, head_dim, mode,
+            bias.has_value() ? &*bias : nullptr, q_w.has_value() ? &*q_w : nullptr, k_w.has_value() ? &*k_w : nullptr, eps,
+            "splitk_rope_cache");
+}
+void read_cache_mx4(at::Tensor& k_out, at::Tensor& v_out, const at::Tensor& k_cache, const at::Tensor& v_cache,
+                    const at::Tensor& slots) {
+  const hipserve::Kv4Cache c = kv4_cache(k_cache, v_cache, k_cache.dim() == 4 ? k_cache.size(1) : 0, "read_cache");
+  const int64_t T = slots.numel();
+  for (const at::Tensor* o : {&k_out, &v_out})
+    TORCH_CHECK(o->device() == k_cache.device() && o->scalar_type() == at::kBFloat16 && o->dim() == 3 && o->size(0) == T &&
+                    o->size(1) == c.nkv && o->size(2) == c.D && (T == 0 || (o->stride(2) == 1 && o->stride(1) == c.D)) &&
+                    (T <= 1 || o->stride(0) >= c.nkv * c.D) && o->stride(0) % 8 == 0 &&
+                    reinterpret_cast<uintptr_t>(o->data_ptr()) % 16 == 0,
+                "read_cache: outputs are bf16 [rows, kv heads, head_dim], a row's heads together, rows at multiples of 16 bytes");
+  TORCH_CHECK(T < (1LL << 30), "read_cache: too many rows");
+  const int64_t* sl = kv4_longs(slots, k_cache, T, "read_cache", "slots");
+  c10::hip::HIPGuardMasqueradingAsCUDA g(k_cache.device());
+  hipserve::launch_kv4_read(k_out.data_ptr(), k_out.stride(0), v_out.data_ptr(), v_out.stride(0), c, sl, (int)T, cur_stream());
+}
+static hipserve::Kv4Attn kv4_attn(at::Tensor& out, const at::Tensor& q, const at::Tensor& k_cache, const at::Tensor& v_cache,
+                                  const at::Tensor& block_tables, int64_t nq, int64_t nkv, double scale, int64_t window,
+                                  int64_t sinks, const char* who) {
+  hipserve::Kv4Attn a{};
+  a.cache = kv4_cache(k_cache, v_cache, nkv, who);
+  TORCH_CHECK(nq > 0 && nq % nkv == 0 && nq / nkv <= 16 && nq < 65536, who, ": nq a multiple of nkv, at most 16 queries per kv head");
+  TORCH_CHECK(window >= 0 && sinks >= 0 && window <= INT32_MAX && sinks <= INT32_MAX, who, ": window >= 0, sinks >= 0");
+  kv4_rows(q, k_cache, nq * a.cache.D, who, "q");
+  kv4_rows(out, k_cache, nq * a.cache.D, who, "out");
+  TORCH_CHECK(block_tables.device() == k_cache.device() && block_tables.scalar_type() == at::kInt && block_tables.dim() == 2 &&
+                  block_tables.stride(1) == 1 && block_tables.stride(0) <= INT32_MAX,
+              who, ": block tables int32 [sequences, blocks]");
+  TORCH_CHECK(block_tables.size(1) * a.cache.block_size <= INT32_MAX - 1024, who, ": contexts of up to 2^31 tokens");
+  a.out = out.data_ptr();
+  a.out_stride = out.stride(0);
+  a.q = q.data_ptr();
+  a.q_stride = q.stride(0);
+  a.block_tables = block_tables.data_ptr<int>();
+  a.bt_stride = block_tables.stride(0);
+  a.bt_width = block_tables.size(1);
+  a.nq = nq;
+  a.scale = (float)scale;
+  a.window = window;
+  a.sinks = window > 0 ? sinks : 0;  // without a window every key is visible
+  return a;
+}
+void paged_decode_mx4(at::Tensor& out, const at::Tensor& q, const at::Tensor& k_cache, const at::Tensor& v_cache,
+                      const at::Tensor& block_tables, const at::Tensor& context_lens, at::Tensor& tmp_out, at::Tensor& tmp_ml,
+                      int64_t nq, int64_t nkv, int64_t part_size, double scale, int64_t window, int64_t sinks,
+                      const c10::optional<at::Tensor>& out16) {
+  const hipserve::Kv4Attn a = kv4_attn(out, q, k_cache, v_cache, block_tables, nq, nkv, scale, window, sinks, "paged_decode");
+  const int64_t B = q.size(0);
+  TORCH_CHECK(out.size(0) >= B && block_tables.size(0) >= B && B < 65536, "paged_decode: rows of out and of the block tables");
+  const int* ctx = kv4_ints(context_lens, k_cache, B, "paged_decode", "context lengths");
+  TORCH_CHECK(part_size > 0 && part_size % 64 == 0 && part_size <= 16384, "paged_decode: partitions of a multiple of 64 tokens, at most 16384");
+  for (const at::Tensor* t : {&tmp_out, &tmp_ml})
+    TORCH_CHECK(t->device() == k_cache.device() && t->scalar_type() == at::kFloat && t->is_contiguous() && t->dim() == 4 &&
+                    t->size(0) >= B && t->size(1) == nq && t->size(2) == tmp_ml.size(2) && t->size(2) > 0 &&
+                    t->size(3) == (t == &tmp_ml ? 2 : a.cache.D),
+                "paged_decode: workspaces fp32 [rows, nq, partitions, head_dim] and [rows, nq, partitions, 2]");
+  TORCH_CHECK(tmp_ml.size(2) * part_size >= block_tables.size(1) * a.cache.block_size,
+              "workspace partitions must cover block_tables capacity");
+  c10::hip::HIPGuardMasqueradingAsCUDA g(k_cache.device());
+  hipserve::launch_kv4_decode(a, ctx, tmp_out.data_ptr<float>(), tmp_ml.data_ptr<float>(), (int)B, (int)part_size,
+                              (int)tmp_ml.size(2), out16_ptr(out16, out), cur_stream());
+}
+void prefill_attention_mx4(at::Tensor& out, const at::Tensor& q, const at::Tensor& k_cache, const at::Tensor& v_cache,
+                           const at::Tensor& block_tables, const at::Tensor& cu_q, const at::Tensor& ctx_lens,
+                           const at::Tensor& tiles, int64_t nq, int64_t nkv, double scale, int64_t window, int64_t sinks) {
+  const hipserve::Kv4Attn a = kv4_attn(out, q, k_cache, v_cache, block_tables, nq, nkv, scale, window, sinks, "prefill_attention");
+  const int64_t seqs = cu_q.numel() - 1;
+  TORCH_CHECK(seqs >= 0 && block_tables.size(0) >= seqs, "prefill_attention: a block table per sequence");
+  TORCH_CHECK(tiles.dim() == 2 && tiles.size(1) == 2, "prefill_attention: tiles [tiles, 2]");
+  const int* cu = kv4_ints(cu_q, k_cache, 1, "prefill_attention", "row offsets");
+  const int* ctx = kv4_ints(ctx_lens, k_cache, seqs, "prefill_attention", "context lengths");
+  const int* tl = kv4_ints(tiles, k_cache, 0, "prefill_attention", "tiles");
+  c10::hip::HIPGuardMasqueradingAsCUDA g(k_cache.device());
+  hipserve::launch_kv4_prefill(a, cu, (int)seqs, ctx, (int)std::min(q.size(0), out.size(0)), tl, (int)tiles.size(0), cur_stream());
+}
+
 // Per-head RMSNorm of q and k inside the merged qkv rows, in place (Qwen3 / Gemma-3).
 void qk_rmsnorm(at::Tensor& qkv, const at::Tensor& q_w, const at::Tensor& k_w, int64_t nq, int64_t nkv,
                 int64_t head_dim, double eps) {
@@ -1320,6 +1475,11 @@ TORCH_LIBRARY(hipserve, m) {
   m.def("silu_and_mul(Tensor(a!) out, Tensor x) -> ()");
   m.def("rope_cache(Tensor(a!) qkv, Tensor positions, Tensor slots, Tensor cos_sin, Tensor(b!) k_cache, Tensor(c!) v_cache, int nq, int nkv, int head_dim, int mode) -> ()");
   m.def("paged_decode(Tensor(a!) out, Tensor q, Tensor k_cache, Tensor v_cache, Tensor block_tables, Tensor context_lens, Tensor(b!) tmp_out, Tensor(c!) tmp_ml, int nq, int nkv, int part_size, float scale, int window=0, Tensor(d!)? out16=None) -> ()");
+  m.def("rope_cache_mx4(Tensor(a!) qkv, Tensor positions, Tensor slots, Tensor cos_sin, Tensor(b!) k_cache, Tensor(c!) v_cache, int nq, int nkv, int head_dim, int mode) -> ()");
+  m.def("splitk_rope_cache_mx4(Tensor(a!) qkv, Tensor ws, int splits, Tensor positions, Tensor slots, Tensor cos_sin, Tensor(b!) k_cache, Tensor(c!) v_cache, int nq, int nkv, int head_dim, int mode, Tensor? bias=None, Tensor? q_w=None, Tensor? k_w=None, float eps=1e-6) -> ()");
+  m.def("read_cache_mx4(Tensor(a!) k_out, Tensor(b!) v_out, Tensor k_cache, Tensor v_cache, Tensor slots) -> ()");
+  m.def("paged_decode_mx4(Tensor(a!) out, Tensor q, Tensor k_cache, Tensor v_cache, Tensor block_tables, Tensor context_lens, Tensor(b!) tmp_out, Tensor(c!) tmp_ml, int nq, int nkv, int part_size, float scale, int window=0, int sinks=0, Tensor(d!)? out16=None) -> ()");
+  m.def("prefill_attention_mx4(Tensor(a!) out, Tensor q, Tensor k_cache, Tensor v_cache, Tensor block_tables, Tensor cu_q, Tensor ctx_lens, Tensor tiles, int nq, int nkv, float scale, int window=0, int sinks=0) -> ()");
   m.def("prefill_attention(Tensor(a!) out, Tensor q, Tensor k_cache, Tensor v_cache, Tensor block_tables, Tensor cu_q, Tensor ctx_lens, Tensor tiles, int nq, int nkv, float scale, int window=0) -> ()");
   m.def("qk_rmsnorm(Tensor(a!) qkv, Tensor q_w, Tensor k_w, int nq, int nkv, int head_dim, float eps) -> ()");
   m.def("gelu_and_mul(Tensor(a!) out, Tensor x) -> ()");
@@ -1385,6 +1545,11 @@ TORCH_LIBRARY_IMPL(hipserve, CUDA, m) {
   m.impl("rope_cache", &rope_cache);
   m.impl("paged_decode", &paged_decode);
   m.impl("prefill_attention", &prefill_attention);
+  m.impl("rope_cache_mx4", &rope_cache_mx4);
+  m.impl("splitk_rope_cache_mx4", &splitk_rope_cache_mx4);
+  m.impl("read_cache_mx4", &read_cache_mx4);
+  m.impl("paged_decode_mx4", &paged_decode_mx4);
+  m.impl("prefill_attention_mx4", &prefill_attention_mx4);
   m.impl("sample", &sample);
   m.impl("penalty_apply", &penalty_apply);
   m.impl("penalty_update", &penalty_update);

@@ -501,7 +501,7 @@ def checkpoint_quantization(model: str) -> str | None:
 
 
 # --kv-cache-dtype values (vLLM's spellings) -> element kind
-KV_CACHE_DTYPES = {"auto": "auto", "bf16": "auto", "bfloat16": "auto", "fp8": "fp8", "fp8_e4m3": "fp8"}
+KV_CACHE_DTYPES = {"auto": "auto", "bf16": "auto", "bfloat16": "auto", "fp8": "fp8", "fp8_e4m3": "fp8", "mxfp4": "mxfp4"}
 
 
 @dataclass(frozen=True)
@@ -529,7 +529,12 @@ class EngineConfig:
     # (OCP e4m3, per-tensor scale 1 as vLLM's --kv-cache-dtype fp8 without calibrated
     # scales: half the KV bytes per token, so 2x the KV blocks and half the decode
     # attention's HBM stream; K / V are rounded to e4m3 when written)
+    # or "mxfp4" (OCP microscaling FP4: e2m1 numbers, a power of two per 32 dims of a token and
+    # head; 4.25 bits, 3.76x the KV blocks of bf16; ops/kv4.py)
     kv_cache_dtype: str = "auto"
+    # sliding-window layers: the first tokens of a sequence that stay visible beside the window
+    # (mxfp4 KV cache; 0 = the window alone, as the model was trained)
+    attention_sinks: int = 0
     host: str = "0.0.0.0"
     port: int = 8080
     extra: dict = field(default_factory=dict)
@@ -541,10 +546,17 @@ class EngineConfig:
             raise ValueError(f"block_size must be a power of two in [16, 256], got {b}")
         if self.kv_cache_dtype not in KV_CACHE_DTYPES:
             raise ValueError(f"kv_cache_dtype must be one of {sorted(KV_CACHE_DTYPES)}, got {self.kv_cache_dtype!r}")
+        if self.attention_sinks < 0 or (self.attention_sinks and not self.kv_mxfp4):
+            raise ValueError(f"attention_sinks must be >= 0 and needs kv_cache_dtype mxfp4, got {self.attention_sinks} "
+                             f"with {self.kv_cache_dtype!r}")
 
     @property
     def kv_fp8(self) -> bool:
         return KV_CACHE_DTYPES[self.kv_cache_dtype] == "fp8"
+
+    @property
+    def kv_mxfp4(self) -> bool:
+        return KV_CACHE_DTYPES[self.kv_cache_dtype] == "mxfp4"
 
     def replace(self, **kw) -> "EngineConfig":
         return dataclasses.replace(self, **kw)

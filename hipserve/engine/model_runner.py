@@ -23,7 +23,7 @@ import torch
 from ..config import EngineConfig, ModelConfig
 from ..models.llama import AttnMeta
 from ..models.registry import build_model, load_weights, model_class
-from ..ops import get_ops
+from ..ops import get_ops, kv4
 from ..parallel.comm import TPGroup
 from ..runtime import native
 from .scheduler import SchedulerOutput
@@ -115,6 +115,13 @@ class ModelRunner:
         if ecfg.kv_fp8:  # e4m3 paged KV cache (the fused qkv -> attention kernel writes bf16 only)
             self.model.kv_dtype = torch.float8_e4m3fn
             self.model.fused_qkv_attention = False
+        if ecfg.kv_mxfp4:
+            if not getattr(self.model, "supports_mxfp4_kv", False):
+                raise ValueError(f"{mcfg.name}: this model has no mxfp4 KV cache")
+            kv4.cache_shape(1, 1, self.block_size, self.model.D)  # refuses a head size that the cache does not hold
+            self.model.kv_dtype = kv4.DTYPE
+            self.model.fused_qkv_attention = False
+            self.model.attention_sinks = ecfg.attention_sinks
         t0 = time.time()
         self._load_weights()
         self.load_time = time.time() - t0

@@ -28,7 +28,7 @@ import torch
 import torch.nn.functional as F
 
 from ..config import ModelConfig
-from ..ops import gemm, pgemm
+from ..ops import gemm, kv4, pgemm
 from ..ops import quant as Q
 from ..ops import reference as ref
 from ..parallel.comm import TPGroup
@@ -121,6 +121,7 @@ class LlamaModel:
     # load FP8 checkpoints natively (e4m3 + scales, ops/quant.py) instead of
     # dequantising them to bf16 at load (weights/safetensors_loader.py)
     native_fp8 = True
+    supports_mxfp4_kv = True  # the 4-bit paged KV cache (ops/kv4.py)
     # fused decode: qkv partials -> RoPE + KV write + attention in one kernel
     # (attention_decode.hip QkvIn), opt-in with HIPSERVE_FUSED_QKV_ATTN=1. Bit-exact.
     # First version: 5.57 vs 5.49 ms per Llama-3-8B B=64 decode step (every wave re-read
@@ -142,7 +143,8 @@ class LlamaModel:
         self.tp = tp
         self.device = torch.device(device)
         self.dtype = dtype
-        self.kv_dtype = dtype  # paged KV cache element (ModelRunner: float8_e4m3fn for --kv-cache-dtype fp8)
+        self.kv_dtype = dtype  # paged KV cache element (ModelRunner: float8_e4m3fn for --kv-cache-dtype fp8, uint8 for mxfp4)
+        self.attention_sinks = 0  # first tokens visible beside a layer's window (ModelRunner: --attention-sinks)
         self.ops = ops
         self.nq, self.nkv, self.inter, self.vpad = shard_sizes(cfg, tp.world_size)
         self.D = cfg.head_dim
@@ -525,7 +527,7 @@ class LlamaModel:
         lw0 = self.layers[0] if self.layers else None
         if (not self.fused_qkv_attention or self.D not in (64, 128) or lw0 is None or lw0.bqkv is not None
                 or (lw0.q_norm is not None and self.cfg.rope_mode != 0)
-                or torch.finfo(self.kv_dtype).bits != 16):
+                or not self.kv_dtype.is_floating_point or torch.finfo(self.kv_dtype).bits != 16):
             return False
         layers = range(len(self.layers)) if layer is None else (layer,)
         return not any(self.cfg.window_of(i) for i in layers)
@@ -661,10 +663,12 @@ class LlamaModel:
                            kc, vc, nq, nkv, D, cfg.rope_mode)
             if Tp:
                 ops.prefill_attention(attn[:Tp], qkv[:Tp], kc, vc, meta.bt_prefill, meta.cu_q,
-                                      meta.ctx_prefill, meta.tiles, nq, nkv, self.scale, win)
+                                      meta.ctx_prefill, meta.tiles, nq, nkv, self.scale, win,
+                                      sinks=self.attention_sinks if win else 0)
             if Td:  # rows past Tp + Td: prefill padding (model_runner._pad_rows)
                 ops.paged_decode(attn[Tp:Tp + Td], qkv[Tp:Tp + Td], kc, vc, meta.bt_decode, meta.ctx_decode,
-                                 tmp_out, tmp_ml, nq, nkv, part, self.scale, win)
+                                 tmp_out, tmp_ml, nq, nkv, part, self.scale, win,
+                                 sinks=self.attention_sinks if win else 0)
             x8 = self._x8p(xn, lw.wgu, glu=True)
             if tp1 and lw.post_attn_norm is None and isinstance(lw.wo, gemm.PackedLinear) and T > 64:
                 gemm.packed_prefill(attn, lw.wo, 1, out=residual)  # residual += o_proj(attn), packed layout
@@ -792,8 +796,8 @@ class LlamaModel:
             elif pt is not None:  # + q/k/v bias and per-head q/k RMSNorm of the family, if any
                 ws, S = pt
                 qkv = torch.empty(T, lw.wqkv.shape[0], device=h.device, dtype=h.dtype)
-                op.splitk_rope_cache(qkv, ws, S, meta.positions, meta.slot_mapping, cs, kc, vc,
-                                     nq, nkv, D, cfg.rope_mode, lw.bqkv, lw.q_norm, lw.k_norm, eps)
+                ops.splitk_rope_cache(qkv, ws, S, meta.positions, meta.slot_mapping, cs, kc, vc,
+                                      nq, nkv, D, cfg.rope_mode, lw.bqkv, lw.q_norm, lw.k_norm, eps)
             else:
                 qkv = self.linear(xn, lw.wqkv)
                 if lw.bqkv is not None:
@@ -804,7 +808,7 @@ class LlamaModel:
                                cfg.rope_mode)
             if pt is None or not fuse_qa:
                 ops.paged_decode(attn, qkv, kc, vc, meta.bt_decode, meta.ctx_decode, tmp_out, tmp_ml,
-                                 nq, nkv, part, self.scale, win, attn16)
+                                 nq, nkv, part, self.scale, win, attn16, sinks=self.attention_sinks if win else 0)
             pt = self._partial(attn, lw.wo, attn16)
             if lw.post_attn_norm is not None:  # Gemma sandwich norm
                 xn16 = self._x16(xn, lw.wgu) if pt is not None else None
@@ -1323,10 +1327,15 @@ class LlamaModel:
 
     # ---------------------------------------------------------------- kv cache
     def kv_bytes_per_block(self, block_size: int) -> int:
-        return 2 * self.cfg.num_layers * self.nkv * block_size * self.D * torch.finfo(self.kv_dtype).bits // 8
+        row = kv4.row_bytes(self.D) if self.kv_dtype == kv4.DTYPE else self.D * torch.finfo(self.kv_dtype).bits // 8
+        return 2 * self.cfg.num_layers * self.nkv * block_size * row
 
     def allocate_kv_cache(self, num_blocks: int, block_size: int):
         L = self.cfg.num_layers
+        if self.kv_dtype == kv4.DTYPE:
+            shape = kv4.cache_shape(num_blocks, self.nkv, block_size, self.D)
+            k, v = (torch.zeros(L, *shape, device=self.device, dtype=kv4.DTYPE) for _ in "kv")
+            return [(k[i], v[i]) for i in range(L)]
         k = torch.zeros(L, num_blocks, self.nkv, block_size, self.D, device=self.device, dtype=self.kv_dtype)
         v = torch.zeros(L, num_blocks, self.nkv, self.D, block_size, device=self.device, dtype=self.kv_dtype)
         return [(k[i], v[i]) for i in range(L)]

@@ -20,6 +20,7 @@ import torch
 import torch.nn.functional as F
 
 from . import gemm
+from . import kv4
 from . import reference as ref
 
 _PKG = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
@@ -241,17 +242,41 @@ class KernelOps:
         self._op.fill_uniform(out, row0, col0, gcols, key, scale)
         return out
 
+    # ---- paged KV cache: bf16, e4m3, or 4 bits (uint8 tensors of ops/kv4.py's layout; csrc/kernels/kv4_*.hip)
     def rope_cache(self, qkv, positions, slots, cos_sin, k_cache, v_cache, nq, nkv, D, mode):
-        self._op.rope_cache(qkv, positions, slots, cos_sin, k_cache, v_cache, nq, nkv, D, mode)
+        """Rotates the queries in place, writes rotated keys and values to their slots (below 0: nowhere; each slot once)."""
+        write = self._op.rope_cache_mx4 if kv4.is_kv4(k_cache) else self._op.rope_cache
+        write(qkv, positions, slots, cos_sin, k_cache, v_cache, nq, nkv, D, mode)
+
+    def splitk_rope_cache(self, qkv, ws, splits, positions, slots, cos_sin, k_cache, v_cache, nq, nkv, D, mode, bias=None,
+                          q_w=None, k_w=None, eps=1e-6):
+        """``rope_cache`` from the split-K partials ws [splits, T, (nq + 2 nkv) D] of the projection; the queries go to qkv."""
+        write = self._op.splitk_rope_cache_mx4 if kv4.is_kv4(k_cache) else self._op.splitk_rope_cache
+        write(qkv, ws, splits, positions, slots, cos_sin, k_cache, v_cache, nq, nkv, D, mode, bias, q_w, k_w, eps)
+
+    def read_cache(self, k_out, v_out, k_cache, v_cache, slots):
+        """Rows of slots of a 4-bit cache as bf16 [T, nkv, D]; zeros for a slot outside of it."""
+        self._op.read_cache_mx4(k_out, v_out, k_cache, v_cache, slots)
 
     def paged_decode(self, out, q, k_cache, v_cache, block_tables, context_lens, tmp_out, tmp_ml,
-                     nq, nkv, part_size, scale, window=0, out16=None):
+                     nq, nkv, part_size, scale, window=0, out16=None, sinks=0):
+        """sinks: first tokens that stay visible beside the window (4-bit cache)."""
+        if kv4.is_kv4(k_cache):
+            self._op.paged_decode_mx4(out, q, k_cache, v_cache, block_tables, context_lens, tmp_out, tmp_ml,
+                                      nq, nkv, part_size, scale, window, sinks, out16)
+            return out
+        ref._no_sinks(sinks)
         self._op.paged_decode(out, q, k_cache, v_cache, block_tables, context_lens, tmp_out, tmp_ml,
                               nq, nkv, part_size, scale, window, out16)
         return out
 
     def prefill_attention(self, out, q, k_cache, v_cache, block_tables, cu_q, ctx_lens, tiles,
-                          nq, nkv, scale, window=0):
+                          nq, nkv, scale, window=0, sinks=0):
+        if kv4.is_kv4(k_cache):
+            self._op.prefill_attention_mx4(out, q, k_cache, v_cache, block_tables, cu_q, ctx_lens, tiles,
+                                           nq, nkv, scale, window, sinks)
+            return out
+        ref._no_sinks(sinks)
         self._op.prefill_attention(out, q, k_cache, v_cache, block_tables, cu_q, ctx_lens, tiles,
                                    nq, nkv, scale, window)
         return out
@@ -1109,20 +1134,19 @@ class ReferenceOps:
         ref.rope_cache(qkv, positions, slots, cos_sin, k_cache, v_cache, nq, nkv, D, mode)
 
     def paged_decode(self, out, q, k_cache, v_cache, block_tables, context_lens, tmp_out, tmp_ml,
-                     nq, nkv, part_size, scale, window=0, out16=None):
-        B = context_lens.shape[0]
-        D = k_cache.shape[3]
-        out[:B, : nq * D].copy_(ref.paged_decode(q, k_cache, v_cache, block_tables, context_lens,
-                                                 nq, nkv, scale, window).view(B, nq * D))
+                     nq, nkv, part_size, scale, window=0, out16=None, sinks=0):
+        got = ref.paged_decode(q, k_cache, v_cache, block_tables, context_lens, nq, nkv, scale, window, sinks).flatten(1)
+        out[: got.shape[0], : got.shape[1]].copy_(got)
         return out
 
     def prefill_attention(self, out, q, k_cache, v_cache, block_tables, cu_q, ctx_lens, tiles,
-                          nq, nkv, scale, window=0):
-        D = k_cache.shape[3]
-        T = int(cu_q[-1])
-        out[:T, : nq * D].copy_(ref.prefill_attention(q, k_cache, v_cache, block_tables, cu_q,
-                                                      ctx_lens, nq, nkv, scale, window).view(T, nq * D))
+                          nq, nkv, scale, window=0, sinks=0):
+        got = ref.prefill_attention(q, k_cache, v_cache, block_tables, cu_q, ctx_lens, nq, nkv, scale, window, sinks).flatten(1)
+        out[: got.shape[0], : got.shape[1]].copy_(got)
         return out
+
+    def read_cache(self, k_out, v_out, k_cache, v_cache, slots):
+        kv4.read_cache(k_out, v_out, k_cache, v_cache, slots)
 
     def penalty_apply(self, logits, slot, pres, freq, rep, counts, seen):
         ref.penalty_apply(logits, slot, pres, freq, rep, counts, seen)

@@ -6,6 +6,7 @@ a GPU). They use exactly the same tensor layouts as the kernels:
 
 * ``k_cache [num_blocks, nkv, block_size, D]``
 * ``v_cache [num_blocks, nkv, D, block_size]`` (transposed per block)
+* 4-bit caches: uint8 ``[num_blocks, nkv, block_size, 17 D / 32]`` (kv4.py)
 * ``cos_sin [max_pos, D]`` = ``[cos(D/2) | sin(D/2)]`` fp32
 """
 from __future__ import annotations
@@ -14,6 +15,8 @@ import math
 
 import numpy as np
 import torch
+
+from . import kv4
 
 
 def rmsnorm(x: torch.Tensor, w: torch.Tensor, eps: float) -> torch.Tensor:
@@ -151,14 +154,24 @@ def rope_cache(qkv, positions, slots, cos_sin, k_cache, v_cache, nq, nkv, D, mod
     v = qkv[:, (nq + nkv) * D:(nq + 2 * nkv) * D].view(T, nkv, D)
     q.copy_(apply_rope(q, positions[:T], cos_sin, mode))
     kr = apply_rope(k, positions[:T], cos_sin, mode)
-    bs = k_cache.shape[2]
     sl = slots[:T].long()
+    if kv4.is_kv4(k_cache):
+        kv4.check(k_cache, v_cache, nkv)
+        kv4.store(k_cache, sl, kr, False)
+        kv4.store(v_cache, sl, v, True)
+        return
+    bs = k_cache.shape[2]
     valid = sl >= 0
     if valid.any():
         sv = sl[valid]
         blk, off = sv // bs, sv % bs
         k_cache[blk, :, off, :] = to_cache(kr[valid], k_cache.dtype)
         v_cache[blk, :, :, off] = to_cache(v[valid], v_cache.dtype)
+
+
+def _no_sinks(sinks: int):
+    if sinks:
+        raise ValueError("first tokens that stay visible beside a window (sinks) need the mxfp4 KV cache")
 
 
 def _gather_kv(k_cache, v_cache, block_table, n):
@@ -171,9 +184,12 @@ def _gather_kv(k_cache, v_cache, block_table, n):
     return k, v
 
 
-def paged_decode(q, k_cache, v_cache, block_tables, context_lens, nq, nkv, scale, window=0):
+def paged_decode(q, k_cache, v_cache, block_tables, context_lens, nq, nkv, scale, window=0, sinks=0):
     """q [B, nq*D (+extra)] -> out [B, nq, D] (fp32 math). window > 0: only the
-    last ``window`` keys (sliding-window layers)."""
+    last ``window`` keys (sliding-window layers) and, of a 4-bit cache, the first ``sinks``."""
+    if kv4.is_kv4(k_cache):
+        return kv4.paged_decode(q, k_cache, v_cache, block_tables, context_lens, nq, nkv, scale, window, sinks)
+    _no_sinks(sinks)
     D = k_cache.shape[3]
     B = context_lens.shape[0]
     G = nq // nkv
@@ -192,9 +208,12 @@ def paged_decode(q, k_cache, v_cache, block_tables, context_lens, nq, nkv, scale
     return out
 
 
-def prefill_attention(q, k_cache, v_cache, block_tables, cu_q, ctx_lens, nq, nkv, scale, window=0):
+def prefill_attention(q, k_cache, v_cache, block_tables, cu_q, ctx_lens, nq, nkv, scale, window=0, sinks=0):
     """q [T, nq*D (+extra)] -> out [T, nq, D]; causal over absolute positions;
-    window > 0: keys within ``window - 1`` positions before the query."""
+    window > 0: keys within ``window - 1`` positions before the query and, of a 4-bit cache, the first ``sinks``."""
+    if kv4.is_kv4(k_cache):
+        return kv4.prefill_attention(q, k_cache, v_cache, block_tables, cu_q, ctx_lens, nq, nkv, scale, window, sinks)
+    _no_sinks(sinks)
     D = k_cache.shape[3]
     G = nq // nkv
     T = int(cu_q[-1])

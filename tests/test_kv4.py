@@ -1,0 +1,767 @@
+"""The 4-bit paged KV cache (--kv-cache-dtype mxfp4): writers, reader, decode and prompt attention with a window and first tokens
+that stay visible, on the CPU engine's operators and (marked gpu) the gfx950 kernels.
+
+The oracle here decodes the cache's bytes from the format's description in 64 bits and attends in 64 bits, without the package's
+code. Bytes and read values must be equal. An attention output may be off by what its roundings to bf16 allow: half a step, 2^-8,
+of each probability (so 2^-8 of the sum of p |v|) and of the output; the 32-bit sums of up to 2048 products before that are
+within 2^-13 of that sum, in the score's exponent included (see ``_check``)."""
+import dataclasses
+import math
+
+import pytest
+import torch
+
+from hipserve.config import PRESETS, EngineConfig
+from hipserve.engine.llm_engine import LLMEngine
+from hipserve.engine.request import SamplingParams
+from hipserve.ops import get_ops, kv4
+from hipserve.ops import reference as ref
+from hipserve.parallel.comm import TPGroup
+
+DEVICES = ["cpu", pytest.param("cuda", marks=pytest.mark.gpu)]
+LEVELS = [0.0, 0.5, 1.0, 1.5, 2.0, 3.0, 4.0, 6.0]
+
+
+# ---------------------------------------------------------------- oracle
+
+def _decode_bytes(cache, values):
+    """[blocks, heads, block_size, D] float64 from the bytes, element by element of the layout's description."""
+    n, h, bs, w = cache.shape
+    d = w * 32 // 17
+    flat = cache.cpu().reshape(n, h, -1)
+    tok, dim = torch.meshgrid(torch.arange(bs), torch.arange(d), indexing="ij")
+    code_at = dim // 2 * bs + tok if values else tok * (d // 2) + dim // 2
+    place = tok if values else tok // 16 * 16 + 4 * (tok % 4) + tok % 16 // 4
+    scale_at = bs * d // 2 + dim // 32 * bs + place
+    pick = lambda at: flat[:, :, at.reshape(-1)].view(n, h, bs, d).long()  # noqa: E731
+    code, byte = pick(code_at) >> (4 * (dim % 2)) & 15, pick(scale_at)
+    y = torch.tensor(LEVELS + [-v for v in LEVELS], dtype=torch.float64)[code] * torch.exp2(byte.double() - 127)
+    return torch.where(byte == 255, float("nan"), y)
+
+
+def _attend(q, k, v, seen, scale):
+    """One head, 64 bits: q [r, D], k and v [n, D], seen [r, n] -> (out [r, D], sum of p |v| [r, D])."""
+    if not (k.isnan().any() or v.isnan().any()):
+        some = seen.any(1, keepdim=True)
+        p = torch.softmax((k @ q.T * scale).T.masked_fill(~seen & some, float("-inf")), 1) * some
+        return p @ v, p @ v.abs()
+    out, size = torch.zeros(len(q), v.shape[1], dtype=torch.float64), torch.zeros(len(q), v.shape[1], dtype=torch.float64)
+    for i in range(len(q)):   # row by row, over the seen keys alone
+        at = seen[i].nonzero().flatten()
+        if len(at):
+            p = torch.softmax(k[at] @ q[i] * scale, 0)
+            out[i], size[i] = p @ v[at], p @ v[at].abs()
+    return out, size
+
+
+def _oracle(q, kc, vc, tables, rows, ctx, nq, nkv, scale, window, sinks):
+    """Sequence i's last rows[i] positions of ctx[i]: (out, size) [sum(rows), nq, D] float64."""
+    keys, vals = _decode_bytes(kc, False), _decode_bytes(vc, True)
+    nb, _, bs, d = keys.shape
+    q, outs, at = q.cpu().double(), [], 0
+    for i, (r, n) in enumerate(zip(rows, ctx)):
+        j = torch.arange(n)
+        page = tables[i].cpu().long()[j // bs] if n else j
+        ok = (page >= 0) & (page < nb)
+        page = torch.where(ok, page, 0)
+        pos = torch.arange(n - r, n)[:, None]
+        seen = (j <= pos) & ok
+        if window:
+            seen &= (j > pos - window) | (j < sinks)
+        heads = [_attend(q[at:at + r, h * d:(h + 1) * d], keys[page, h // (nq // nkv), j % bs], vals[page, h // (nq // nkv), j % bs],
+                         seen, scale) for h in range(nq)]
+        outs.append([torch.stack(x, 1) for x in zip(*heads)])
+        at += r
+    return [torch.cat(x) for x in zip(*outs)]
+
+
+def _check(got, want, size):
+    """A probability is rounded to bf16 once and the output once: 2^-8 of each. Scores are sums of 32 bits of up to 128 products of a few
+    units, off by under 2^-14 in the exponent, and the sums over the keys add less: together under 2^-11 of the sum of p |v|."""
+    got = got.float().cpu().double().view(want.shape)
+    assert torch.equal(got.isnan(), want.isnan())
+    off = (got - want).abs()
+    tol = (2 ** -8 + 2 ** -11) * size + 2 ** -8 * want.abs() + 1e-30
+    bad = (off > tol) & ~want.isnan()
+    assert not bad.any(), f"off by {(off / tol)[~want.isnan()].max():.3f} of what the roundings allow"
+
+
+# ---------------------------------------------------------------- inputs
+
+def _random_cache(gen, nb, nkv, bs, d, spread=3):
+    """Caches of any codes and of scales around 1."""
+    shape = kv4.cache_shape(nb, nkv, bs, d)
+    out = []
+    for _ in "kv":
+        c = torch.randint(0, 256, shape, generator=gen, dtype=torch.uint8).view(nb, nkv, -1)
+        c[..., bs * d // 2:] = torch.randint(125 - spread, 125 + spread, (nb, nkv, bs * d // 32), generator=gen).to(torch.uint8)
+        out.append(c.view(shape))
+    return out
+
+
+def _tables(gen, ctx, bs, width=None):
+    need = [max(1, -(-n // bs)) for n in ctx]
+    width = width or max(need)
+    nb = sum(need) + 2
+    ids = torch.randperm(nb, generator=gen).int()
+    t = torch.zeros(len(ctx), width, dtype=torch.int32)
+    at = 0
+    for i, n in enumerate(need):
+        t[i, :n] = ids[at:at + n]
+        at += n
+    return nb, t
+
+
+def _decode(ops, dev, q, kc, vc, bt, ctx, nq, nkv, d, bs, part, window, sinks, out=None, out16=None):
+    b = q.shape[0]
+    parts = max(1, -(-bt.shape[1] * bs // part))
+    to, tm = torch.full((b, nq, parts, d), float("nan"), device=dev), torch.full((b, nq, parts, 2), float("nan"), device=dev)
+    out = torch.full((b, nq * d), float("nan"), device=dev, dtype=torch.bfloat16) if out is None else out
+    kw = {} if out16 is None else dict(out16=out16)
+    ops.paged_decode(out, q.to(dev), kc.to(dev), vc.to(dev), bt.to(dev), torch.as_tensor(ctx, dtype=torch.int32).to(dev), to, tm, nq, nkv,
+                     part, 1 / math.sqrt(d), window, sinks=sinks, **kw)
+    return out
+
+
+def _tiles(rows):
+    return torch.tensor([(i, r) for i, n in enumerate(rows) for r in range(0, n, 128)], dtype=torch.int32).view(-1, 2)
+
+
+def _prompt(ops, dev, q, kc, vc, bt, rows, ctx, nq, nkv, d, window, sinks, out=None):
+    cu = torch.tensor([sum(rows[:i]) for i in range(len(rows) + 1)], dtype=torch.int32)
+    out = torch.full((q.shape[0], nq * d), float("nan"), device=dev, dtype=torch.bfloat16) if out is None else out
+    ops.prefill_attention(out, q.to(dev), kc.to(dev), vc.to(dev), bt.to(dev), cu.to(dev), torch.tensor(ctx, dtype=torch.int32).to(dev),
+                          _tiles(rows).to(dev), nq, nkv, 1 / math.sqrt(d), window, sinks=sinks)
+    return out
+
+
+def _queries(gen, rows, nq, nkv, d):
+    """Rows of a merged projection, as the engine passes them."""
+    return torch.randn(rows, (nq + 2 * nkv) * d, generator=gen).to(torch.bfloat16)
+
+
+# ---------------------------------------------------------------- the format
+
+def test_quantise_takes_the_nearest_level():
+    """Every value is within half a step of its neighbours on the grid, or beyond the largest level by at most a sixth; ties go to
+    the even code."""
+    gen = torch.Generator().manual_seed(0)
+    x = (torch.randn(512, 96, generator=gen) * torch.exp2(torch.randint(-60, 60, (512, 1), generator=gen).float())).to(torch.bfloat16)
+    codes, scales = kv4.quantise(x)
+    s = torch.exp2(scales.double() - 127).repeat_interleave(32, -1)
+    levels = torch.tensor(LEVELS, dtype=torch.float64)
+    a = x.double().abs() / s
+    assert a.max() <= 7 and (a.unflatten(-1, (-1, 32)).amax(-1) > 3).all()
+    dist = (a[..., None] - levels).abs()
+    assert torch.equal(dist.gather(-1, (codes & 7).long()[..., None]).squeeze(-1), dist.min(-1).values)
+    tied = (dist == dist.min(-1, keepdim=True).values).sum(-1) == 2
+    assert tied.any() and not (codes[tied] & 1).any()
+    assert torch.equal(codes >= 8, torch.signbit(x))
+    assert torch.equal(kv4.dequantise(codes, scales).double(), torch.where(codes >= 8, -1.0, 1.0) * levels[(codes & 7).long()] * s)
+
+
+def test_quantise_at_the_ends_of_the_range():
+    big = torch.finfo(torch.bfloat16).max
+    x = torch.zeros(7, 64, dtype=torch.bfloat16)
+    x[0, 3] = big                     # reads as 6 * 2^125
+    x[1, 3] = 2.0 ** -133             # below half of the smallest value, 2^-120: zero
+    x[2, 3] = 2.0 ** -118
+    x[3, 3], x[3, 40] = float("nan"), 2.0
+    x[4, 3], x[4, 40] = float("-inf"), -3.0
+    x[5, 3] = 7.0                     # exactly 7 units: stays under the smaller scale and reads as 6
+    x[6, 3] = 7.03125                 # the next bf16: the scale doubles
+    codes, scales = kv4.quantise(x)
+    y = kv4.dequantise(codes, scales)
+    assert scales[:, 0].tolist() == [252, 8, 9 - 1, 255, 255, 127, 128]
+    assert y[0, 3] == 6 * 2.0 ** 125 and y[1].abs().max() == 0 and y[2, 3] == 2.0 ** -118
+    assert y[3:5, :32].isnan().all() and y[3, 40] == 2 and y[4, 40] == -3 and not codes[3:5, :32].any()
+    assert y[5, 3] == 6 and y[6, 3] == 8 and not y.isinf().any()
+
+
+# ---------------------------------------------------------------- writing and reading
+
+def _values(gen, t, n):
+    x = torch.randn(t, n, generator=gen)
+    x[:, 5::48] *= 6
+    return x.to(torch.bfloat16)
+
+
+@pytest.mark.parametrize("dev", DEVICES)
+@pytest.mark.parametrize("mode", [0, 1])
+@pytest.mark.parametrize("nq,nkv,d,bs", [(32, 8, 128, 16), (5, 5, 96, 32), (14, 2, 64, 64), (3, 1, 128, 256)])
+@pytest.mark.parametrize("t,order", [(1, "in order"), (37, "anywhere"), (131, "in order"), (260, "aligned")])
+def test_write_holds_the_quantised_rows(dev, mode, nq, nkv, d, bs, t, order):
+    """The cache's bytes are those of the rows that a bf16 cache holds after the same call, quantised, every other byte is left, and
+    the queries are rotated to the same bits; rows in a wider buffer, slots below 0 and behind the cache."""
+    gen = torch.Generator().manual_seed(t + d)
+    ops, nb = get_ops(dev), 2 + 600 // bs
+    wide = _values(gen, t, (nq + 2 * nkv) * d + 16).to(dev)
+    pos = torch.randint(0, 4000, (t,), generator=gen).to(dev)
+    slots = {"anywhere": torch.randperm(nb * bs, generator=gen)[:t], "in order": torch.arange(t) + bs + 5,
+             "aligned": torch.arange(t) + bs}[order].to(dev)
+    if t > 20:
+        slots[3], slots[17] = -1, nb * bs
+    cs = ref.rope_cos_sin(d, 4096, 500000.0).to(dev)
+    kc, vc = (c.to(dev) for c in _random_cache(gen, nb, nkv, bs, d))
+    before = kc.clone(), vc.clone()
+    kb = torch.zeros(nb + 1, nkv, bs, d, device=dev, dtype=torch.bfloat16)
+    vb = torch.zeros(nb + 1, nkv, d, bs, device=dev, dtype=torch.bfloat16)
+    plain, rows = wide.clone(), wide.clone()
+    cols = (nq + 2 * nkv) * d
+    ops.rope_cache(plain[:, :cols], pos, slots, cs, kb, vb, nq, nkv, d, mode)
+    ops.rope_cache(rows[:, :cols], pos, slots, cs, kc, vc, nq, nkv, d, mode)
+    assert torch.equal(rows[:, : nq * d], plain[:, : nq * d])
+    assert torch.equal(rows[:, nq * d:], wide[:, nq * d:])
+    ok = (slots >= 0) & (slots < nb * bs)
+    s = slots[ok].cpu()
+    want = before[0].cpu(), before[1].cpu()
+    for c, rows_of, values in zip(want, (kb[slots[ok] // bs, :, slots[ok] % bs], vb[slots[ok] // bs, :, :, slots[ok] % bs]), (False, True)):
+        codes, scales = kv4.quantise(rows_of.cpu())
+        flat = c.view(nb, nkv, -1)
+        for i, sl in enumerate(s.tolist()):   # byte by byte of the layout's description
+            o, hb = sl % bs, flat[sl // bs]
+            packed = codes[i, :, 0::2] | (codes[i, :, 1::2] << 4)
+            if values:
+                hb[:, o:bs * d // 2:bs] = packed
+                hb[:, bs * d // 2 + o::bs] = scales[i]
+            else:
+                hb[:, o * d // 2:(o + 1) * d // 2] = packed
+                hb[:, bs * d // 2 + o // 16 * 16 + 4 * (o % 4) + o % 16 // 4::bs] = scales[i]
+    assert torch.equal(kc.cpu(), want[0]) and torch.equal(vc.cpu(), want[1])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("t,splits", [(1, 1), (5, 3), (64, 8), (100, 17)])
+@pytest.mark.parametrize("extra", ["plain", "bias", "norm", "neighbours"])
+@pytest.mark.parametrize("nq,nkv,d", [(32, 8, 128), (14, 2, 64), (6, 6, 96)])
+def test_write_of_partials(t, splits, extra, nq, nkv, d):
+    """From a decode step's split-K partials: as the bf16 cache's writer, rounding for rounding."""
+    if extra == "norm" and d == 96:
+        pytest.skip("no writer takes norms of heads of 96")
+    gen = torch.Generator().manual_seed(t)
+    ops, bs, nb = get_ops("cuda"), 16, 40
+    n = (nq + 2 * nkv) * d
+    ws = torch.randn(splits, t, n, generator=gen).cuda()
+    pos, slots = torch.randint(0, 4000, (t,), generator=gen).cuda(), torch.randperm(nb * bs, generator=gen)[:t].cuda()
+    cs = ref.rope_cos_sin(d, 4096, 10000.0).cuda()
+    opts = dict(bias=torch.randn(n, generator=gen).to(torch.bfloat16).cuda()) if extra == "bias" else {}
+    if extra == "norm":
+        opts = dict(q_w=torch.rand(d, generator=gen).cuda() + 0.5, k_w=torch.rand(d, generator=gen).cuda() + 0.5, eps=1e-6)
+    kb = torch.zeros(nb, nkv, bs, d, device="cuda", dtype=torch.bfloat16)
+    vb = torch.zeros(nb, nkv, d, bs, device="cuda", dtype=torch.bfloat16)
+    kc, vc = (torch.zeros(kv4.cache_shape(nb, nkv, bs, d), device="cuda", dtype=torch.uint8) for _ in "kv")
+    got, want = (torch.zeros(t, n, device="cuda", dtype=torch.bfloat16) for _ in "gw")
+    mode = 1 if extra == "neighbours" else 0
+    ops.splitk_rope_cache(want, ws, splits, pos, slots, cs, kb, vb, nq, nkv, d, mode, **opts)
+    ops.splitk_rope_cache(got, ws, splits, pos, slots, cs, kc, vc, nq, nkv, d, mode, **opts)
+    assert torch.equal(got[:, : nq * d], want[:, : nq * d])
+    for cache, rows, values in ((kc, kb[slots // bs, :, slots % bs], False), (vc, vb[slots // bs, :, :, slots % bs], True)):
+        fresh = torch.zeros_like(cache)
+        kv4.store(fresh, slots, rows, values)
+        assert torch.equal(cache, fresh)
+
+
+@pytest.mark.gpu
+def test_write_quantises_every_bf16_value_as_the_reference():
+    """All 65536 values of bf16, NaNs and infinities among them, in groups of neighbours and of strangers, as V rows."""
+    ops, nkv, d, bs = get_ops("cuda"), 8, 128, 16
+    bits = torch.arange(65536, dtype=torch.int32)
+    gen = torch.Generator().manual_seed(3)
+    for order in (bits, bits[torch.randperm(65536, generator=gen)], (bits & 0x8000) | 0x3c00 | (bits * 7 & 0x3ff)):
+        v = order.to(torch.int16).view(torch.bfloat16).view(-1, nkv * d).cuda()
+        t = v.shape[0]
+        qkv = torch.cat((torch.zeros(t, nkv * d, device="cuda", dtype=torch.bfloat16), v), 1)
+        kc, vc = (torch.zeros(kv4.cache_shape(8, nkv, bs, d), device="cuda", dtype=torch.uint8) for _ in "kv")
+        slots = torch.arange(t, device="cuda") + 16
+        cs = ref.rope_cos_sin(d, 16, 10000.0).cuda()
+        ops.rope_cache(qkv, torch.zeros(t, device="cuda", dtype=torch.long), slots, cs, kc, vc, 0, nkv, d, 0)
+        want = torch.zeros(vc.shape, dtype=torch.uint8)
+        kv4.store(want, slots.cpu(), v.view(t, nkv, d).cpu(), True)
+        assert torch.equal(vc.cpu(), want)
+        k, v2 = (torch.empty(t, nkv, d, device="cuda", dtype=torch.bfloat16) for _ in "kv")
+        ops.read_cache(k, v2, kc, vc, slots)
+        assert torch.equal(v2.cpu().float().nan_to_num(7.0), kv4.load(want, slots.cpu(), True).float().nan_to_num(7.0))
+
+
+@pytest.mark.parametrize("dev", DEVICES)
+@pytest.mark.parametrize("nkv,d,bs", [(8, 128, 16), (3, 96, 32), (2, 64, 128)])
+@pytest.mark.parametrize("t,order", [(0, "in order"), (1, "anywhere"), (16, "aligned"), (100, "anywhere"), (333, "in order")])
+def test_read_gives_the_values(dev, nkv, d, bs, t, order):
+    gen = torch.Generator().manual_seed(t + bs)
+    nb = 2 + 400 // bs
+    kc, vc = _random_cache(gen, nb, nkv, bs, d, spread=60)
+    kc.view(nb, nkv, -1)[1, 0, bs * d // 2 + 3] = 255
+    vc.view(nb, nkv, -1)[1, 0, bs * d // 2 + 5] = 255
+    slots = {"anywhere": torch.randint(0, nb * bs, (t,), generator=gen), "in order": torch.arange(t) + 7,
+             "aligned": torch.arange(t) + bs}[order]
+    if t > 20:
+        slots[2], slots[19], slots[20] = -1, nb * bs, slots[5]   # a slot read twice
+    k, v = (torch.full((t + 1, nkv * d + 8), 7.0, dtype=torch.bfloat16, device=dev) for _ in "kv")
+    ko, vo = (x[:t, :nkv * d].unflatten(1, (nkv, d)) for x in (k, v))
+    get_ops(dev).read_cache(ko, vo, kc.to(dev), vc.to(dev), slots.to(dev))
+    ok = (slots >= 0) & (slots < nb * bs)
+    at = torch.where(ok, slots, 0)
+    for got, cache, values in ((ko, kc, False), (vo, vc, True)):
+        want = torch.where(ok[:, None, None], _decode_bytes(cache, values)[at // bs, :, at % bs], 0.0)
+        assert torch.equal(got.cpu().double().nan_to_num(12345.0), want.nan_to_num(12345.0))
+    assert (k[t] == 7).all() and (k[:, nkv * d:] == 7).all()
+
+
+# ---------------------------------------------------------------- attention
+
+HEADS = [(32, 8, 128, 16), (16, 1, 128, 64), (7, 7, 96, 16), (28, 4, 64, 32), (12, 4, 96, 256)]
+WINDOWS = [(0, 0), (100, 0), (100, 4), (64, 70), (1, 1), (1000, 3), (200, 150)]
+
+
+@pytest.mark.parametrize("dev", DEVICES)
+@pytest.mark.parametrize("nq,nkv,d,bs", HEADS)
+@pytest.mark.parametrize("window,sinks", WINDOWS)
+@pytest.mark.parametrize("part", [64, 512])
+def test_decode(dev, nq, nkv, d, bs, window, sinks, part):
+    """Lengths from none to many partitions, odd ones, ones that end inside a page and a chunk; a row of no keys is zeros."""
+    gen = torch.Generator().manual_seed(nq + part)
+    ctx = [1, 0, 15, 16, 17, 63, 64, 65, 130, 600, 1300, 257]
+    nb, bt = _tables(gen, ctx, bs)
+    kc, vc = _random_cache(gen, nb, nkv, bs, d)
+    q = _queries(gen, len(ctx), nq, nkv, d)
+    got = _decode(get_ops(dev), dev, q, kc, vc, bt, ctx, nq, nkv, d, bs, part, window, sinks)
+    want, size = _oracle_rows(q, kc, vc, bt, ctx, nq, nkv, d, window, sinks)
+    _check(got, want, size)
+    assert not got[1].any()
+
+
+def _oracle_rows(q, kc, vc, bt, ctx, nq, nkv, d, window, sinks):
+    """One row a sequence, zeros for those without keys."""
+    live = [i for i, n in enumerate(ctx) if n]
+    w, s = _oracle(q[live], kc, vc, bt[live], [1] * len(live), [ctx[i] for i in live], nq, nkv, 1 / math.sqrt(d), window, sinks)
+    out = [torch.zeros(len(ctx), nq, d, dtype=torch.float64) for _ in "ws"]
+    out[0][live], out[1][live] = w, s
+    return out
+
+
+SEQS = [([1], [1]), ([5, 40, 1, 130], [5, 300, 64, 130]), ([64, 128, 33], [64, 129, 500]), ([257, 3], [321, 1000])]
+
+
+@pytest.mark.parametrize("dev", DEVICES)
+@pytest.mark.parametrize("nq,nkv,d,bs", HEADS + [(6, 2, 128, 16), (8, 1, 64, 16), (10, 2, 128, 16)])
+@pytest.mark.parametrize("window,sinks", WINDOWS)
+@pytest.mark.parametrize("rows,ctx", SEQS)
+def test_prompt(dev, nq, nkv, d, bs, window, sinks, rows, ctx):
+    """Whole prompts and portions behind cached tokens; the rows behind the last sequence are left as they were."""
+    if dev == "cpu" and (nq, window) in ((32, 1000), (16, 64), (28, 100)):
+        pytest.skip("covered by the other heads")
+    gen = torch.Generator().manual_seed(nq + sum(rows))
+    nb, bt = _tables(gen, ctx, bs)
+    kc, vc = _random_cache(gen, nb, nkv, bs, d)
+    q = _queries(gen, sum(rows) + 3, nq, nkv, d)
+    out = torch.full((sum(rows) + 3, nq * d + 8), 3.0, device=dev, dtype=torch.bfloat16)
+    _prompt(get_ops(dev), dev, q, kc, vc, bt, rows, ctx, nq, nkv, d, window, sinks, out=out[:, :nq * d])
+    want, size = _oracle(q, kc, vc, bt, rows, ctx, nq, nkv, 1 / math.sqrt(d), window, sinks)
+    _check(out[:sum(rows), :nq * d].reshape(-1, nq, d), want, size)
+    assert (out[sum(rows):] == 3).all() and (out[:, nq * d:] == 3).all()
+
+
+@pytest.mark.parametrize("dev", DEVICES)
+@pytest.mark.parametrize("d", [64, 96, 128])
+@pytest.mark.parametrize("window,sinks", [(0, 0), (40, 4)])
+def test_hidden_nans_stay_hidden_and_seen_ones_show(dev, d, window, sinks):
+    """Groups of scale byte 255 (a NaN was written) in tokens behind a row, before its window and behind the context never reach it;
+    where a row sees one, a key makes the whole row NaN, a value the 32 dims of its group."""
+    gen = torch.Generator().manual_seed(d)
+    nq, nkv, bs, n = 4, 2, 16, 150
+    nb, bt = _tables(gen, [n, n], bs)
+    kc, vc = _random_cache(gen, nb, nkv, bs, d)
+
+    def spoil(cache, seq, tok, head, group, values):
+        o = tok % bs
+        place = o if values else 4 * (o % 4) + o // 4
+        cache.view(nb, nkv, -1)[int(bt[seq, tok // bs]), head, bs * d // 2 + group * bs + place] = 255
+
+    for seq, tok, head, group in ((0, 70, 0, 1), (0, 101, 1, 0), (1, 149, 0, 0), (0, 2, 0, d // 32 - 1)):
+        spoil(vc, seq, tok, head, group, True)
+    for seq, tok, head, group in ((0, 120, 1, 0), (1, 60, 0, d // 32 - 1)):
+        spoil(kc, seq, tok, head, group, False)
+    for tok in range(n, -(-n // bs) * bs):   # what is left of the last pages
+        for seq in (0, 1):
+            for g in range(d // 32):
+                for h in range(nkv):
+                    spoil(kc, seq, tok, h, g, False)
+                    spoil(vc, seq, tok, h, g, True)
+    rows = [n, 100]
+    q = _queries(gen, sum(rows), nq, nkv, d)
+    got = _prompt(get_ops(dev), dev, q, kc, vc, bt, rows, [n, n], nq, nkv, d, window, sinks)
+    want, size = _oracle(q, kc, vc, bt, rows, [n, n], nq, nkv, 1 / math.sqrt(d), window, sinks)
+    assert want.isnan().any() and not want.isnan().all()
+    _check(got.view(-1, nq, d), want, size)
+    lens = [n, n, 60, 71, 101, 121, 1]
+    pick = [0, 1, 1, 0, 0, 0, 0]
+    for part in (64, 256):
+        got = _decode(get_ops(dev), dev, q[:7], kc, vc, bt[pick], lens, nq, nkv, d, bs, part, window, sinks)
+        want, size = _oracle(q[:7], kc, vc, bt[pick], [1] * 7, lens, nq, nkv, 1 / math.sqrt(d), window, sinks)
+        _check(got.view(-1, nq, d), want, size)
+
+
+@pytest.mark.parametrize("dev", DEVICES)
+def test_pages_outside_of_the_cache_are_not_seen(dev):
+    """Block ids below 0 and behind the cache: their keys are hidden, a row without any other is zeros; a context longer than its
+    table ends with the table."""
+    gen = torch.Generator().manual_seed(5)
+    nq, nkv, d, bs = 8, 2, 128, 16
+    ctx = [200, 90, 40, 33]
+    nb, bt = _tables(gen, ctx, bs)
+    kc, vc = _random_cache(gen, nb, nkv, bs, d)
+    bt[0, 3], bt[0, 12], bt[1, 0], bt[2, :] = -1, nb, 2 ** 31 - 1, -7
+    q = _queries(gen, 204, nq, nkv, d)
+    got = _decode(get_ops(dev), dev, q[:4], kc, vc, bt, ctx, nq, nkv, d, bs, 64, 0, 0)
+    want, size = _oracle(q[:4], kc, vc, bt, [1] * 4, ctx, nq, nkv, 1 / math.sqrt(d), 0, 0)
+    _check(got.view(4, nq, d), want, size)
+    assert not got[2].any()
+    rows = [130, 40, 1, 33]
+    got = _prompt(get_ops(dev), dev, q, kc, vc, bt, rows, ctx, nq, nkv, d, 50, 4)
+    want, size = _oracle(q, kc, vc, bt, rows, ctx, nq, nkv, 1 / math.sqrt(d), 50, 4)
+    _check(got[:204].view(204, nq, d), want, size)
+    long = torch.tensor([10 ** 6, 90, 40, 33], dtype=torch.int32)
+    got = _decode(get_ops(dev), dev, q[:4], kc, vc, bt, long, nq, nkv, d, bs, 64, 0, 0)
+    want, size = _oracle(q[:4], kc, vc, bt, [1] * 4, [bt.shape[1] * bs, 90, 40, 33], nq, nkv, 1 / math.sqrt(d), 0, 0)
+    _check(got.view(4, nq, d), want, size)
+
+
+@pytest.mark.parametrize("dev", DEVICES)
+def test_sharp_softmax_and_far_keys(dev):
+    """Queries so large that one key takes all, keys of very different scales: the running maximum moves far, early and late."""
+    gen = torch.Generator().manual_seed(11)
+    nq, nkv, d, bs, n = 8, 2, 128, 16, 700
+    nb, bt = _tables(gen, [n, n], bs)
+    kc, vc = _random_cache(gen, nb, nkv, bs, d, spread=5)
+    q = _queries(gen, 400, nq, nkv, d) * 20
+    got = _decode(get_ops(dev), dev, q[:2], kc, vc, bt, [n, n - 1], nq, nkv, d, bs, 128, 0, 0)
+    want, size = _oracle(q[:2], kc, vc, bt, [1, 1], [n, n - 1], nq, nkv, 1 / math.sqrt(d), 0, 0)
+    # scores of up to 2^11: 32-bit sums of them are off by 2^-12, and so is the exponent
+    _check_sharp(got.view(2, nq, d), want, size)
+    got = _prompt(get_ops(dev), dev, q, kc, vc, bt, [300, 100], [n, n], nq, nkv, d, 0, 0)
+    want, size = _oracle(q, kc, vc, bt, [300, 100], [n, n], nq, nkv, 1 / math.sqrt(d), 0, 0)
+    _check_sharp(got.view(400, nq, d), want, size)
+
+
+def _check_sharp(got, want, size):
+    """Scores reach some thousands here: a sum of 128 products in 32 bits is off by up to 2^-24 of the sum of their magnitudes a step,
+    2^-24 * 128 * 2^13 = 2^-4 at worst, 2^-8 for errors of either sign; a probability is off by as much, 2^-7 with the two scores of a ratio."""
+    off = (got.float().cpu().double() - want).abs()
+    assert (off <= (2 ** -8 + 2 ** -7) * 2 * size + 2 ** -8 * want.abs() + 1e-30).all()
+
+
+@pytest.mark.gpu
+def test_decode_writes_the_f16_copy():
+    gen = torch.Generator().manual_seed(2)
+    nq, nkv, d, bs, ctx = 16, 4, 128, 16, [700, 1, 0, 300]
+    nb, bt = _tables(gen, ctx, bs)
+    kc, vc = _random_cache(gen, nb, nkv, bs, d)
+    q = _queries(gen, 4, nq, nkv, d)
+    for part in (128, 1024):
+        out16 = torch.full((4, nq * d), float("nan"), device="cuda", dtype=torch.float16)
+        out = _decode(get_ops("cuda"), "cuda", q, kc, vc, bt, ctx, nq, nkv, d, bs, part, 0, 0, out16=out16)
+        h = out.float().to(torch.float16).view(4, -1, 8)[:, :, [0, 2, 1, 3, 4, 6, 5, 7]].reshape(4, -1)
+        assert torch.equal(out16, h)
+
+
+@pytest.mark.gpu
+@pytest.mark.slow
+def test_offsets_past_32_bits():
+    """A cache of over 2^32 bytes a tensor: blocks at its end are written, read and attended to like the first ones."""
+    nq, nkv, d, bs = 8, 8, 128, 16
+    nb = (1 << 32) // (nkv * kv4.row_bytes(d) * bs) + 600
+    kc, vc = (torch.empty(kv4.cache_shape(nb, nkv, bs, d), device="cuda", dtype=torch.uint8) for _ in "kv")
+    assert kc.numel() > 1 << 32
+    ops, n = get_ops("cuda"), 200
+    gen = torch.Generator().manual_seed(1)
+    qkv = _values(gen, n, (nq + 2 * nkv) * d).cuda()
+    cs = ref.rope_cos_sin(d, 512, 10000.0).cuda()
+    got = []
+    for first in (0, nb - 13):
+        bt = torch.arange(first, first + 13, device="cuda", dtype=torch.int32)[None]
+        rows, pos = qkv.clone(), torch.arange(n, device="cuda")
+        slots = first * bs + pos
+        ops.rope_cache(rows, pos, slots, cs, kc, vc, nq, nkv, d, 0)
+        k, v = (torch.empty(n, nkv, d, device="cuda", dtype=torch.bfloat16) for _ in "kv")
+        ops.read_cache(k, v, kc, vc, slots)
+        out, one = torch.empty(n, nq * d, device="cuda", dtype=torch.bfloat16), torch.empty(1, nq * d, device="cuda", dtype=torch.bfloat16)
+        ints = lambda *x: torch.tensor(x, device="cuda", dtype=torch.int32)  # noqa: E731
+        ops.prefill_attention(out, rows, kc, vc, bt, ints(0, n), ints(n), _tiles([n]).cuda(), nq, nkv, 0.09, 0)
+        ws = torch.empty(1, nq, 2, d, device="cuda"), torch.empty(1, nq, 2, 2, device="cuda")
+        ops.paged_decode(one, rows[-1:], kc, vc, bt, ints(n), *ws, nq, nkv, 128, 0.09, 0)
+        got.append((k, v, out, one))
+    assert all(torch.equal(a, b) for a, b in zip(*got)) and got[0][2].float().abs().sum() > 0
+
+
+# ---------------------------------------------------------------- together, as a step uses them
+
+@pytest.mark.parametrize("dev", DEVICES)
+def test_a_sequence_from_prompt_to_decode(dev):
+    """A prompt in two portions, then tokens one by one: writes, prompt and decode attention share one cache; every output is the
+    oracle's over the bytes, and a token attends to the same values whichever operator reads them."""
+    gen = torch.Generator().manual_seed(9)
+    nq, nkv, d, bs, n, window, sinks = 8, 2, 128, 16, 150, 60, 4
+    ops = get_ops(dev)
+    nb, bt = _tables(gen, [n + 10], bs)
+    kc, vc = (torch.zeros(kv4.cache_shape(nb, nkv, bs, d), dtype=torch.uint8, device=dev) for _ in "kv")
+    cs = ref.rope_cos_sin(d, 512, 10000.0).to(dev)
+    x = _values(gen, n + 10, (nq + 2 * nkv) * d)
+    scale = 1 / math.sqrt(d)
+    at = 0
+    for rows in [100, 50] + [1] * 10:
+        step = x[at:at + rows].clone().to(dev)
+        pos = torch.arange(at, at + rows)
+        slots = bt[0, pos // bs].long() * bs + pos % bs
+        ops.rope_cache(step, pos.to(dev), slots.to(dev), cs, kc, vc, nq, nkv, d, 0)
+        at += rows
+        if rows > 1:
+            got = _prompt(ops, dev, step, kc, vc, bt, [rows], [at], nq, nkv, d, window, sinks)
+        else:
+            got = _decode(ops, dev, step, kc, vc, bt, [at], nq, nkv, d, bs, 64, window, sinks)
+            again = _prompt(ops, dev, step, kc, vc, bt, [1], [at], nq, nkv, d, window, sinks)
+        want, size = _oracle(step, kc, vc, bt, [rows], [at], nq, nkv, scale, window, sinks)
+        _check(got.view(rows, nq, d), want, size)
+        if rows == 1:
+            _check(again.view(1, nq, d), want, size)
+    k, v = (torch.empty(n, nkv, d, dtype=torch.bfloat16, device=dev) for _ in "kv")
+    pos = torch.arange(n)
+    ops.read_cache(k, v, kc, vc, (bt[0, pos // bs].long() * bs + pos % bs).to(dev))
+    assert torch.equal(v.cpu(), kv4.dequantise(*kv4.quantise(x[:n, (nq + nkv) * d:].view(n, nkv, d))))
+
+
+@pytest.mark.gpu
+def test_captured_steps_replay():
+    """A decode step's write and attention and a prompt's, captured once, replayed for new rows, lengths and tables with eager work in
+    between; two graphs that share the workspace, on a side stream."""
+    gen = torch.Generator().manual_seed(4)
+    nq, nkv, d, bs, b = 8, 2, 128, 16, 6
+    ops, n = get_ops("cuda"), (8 + 4) * 128
+    nb, width = 200, 16
+    kc, vc = (c.cuda() for c in _random_cache(gen, nb, nkv, bs, d))
+    cs = ref.rope_cos_sin(d, 512, 10000.0).cuda()
+    qkv, pos = torch.zeros(b, n, device="cuda", dtype=torch.bfloat16), torch.zeros(b, device="cuda", dtype=torch.long)
+    slots, ctx = torch.zeros(b, device="cuda", dtype=torch.long), torch.ones(b, device="cuda", dtype=torch.int32)
+    bt = torch.zeros(b, width, device="cuda", dtype=torch.int32)
+    to, tm = torch.empty(b, nq, 4, d, device="cuda"), torch.empty(b, nq, 4, 2, device="cuda")
+    out, out_p = (torch.empty(b, nq * d, device="cuda", dtype=torch.bfloat16) for _ in "dp")
+    cu, tiles = torch.tensor([0, b], device="cuda", dtype=torch.int32), _tiles([b]).cuda()
+
+    def decode():
+        ops.rope_cache(qkv, pos, slots, cs, kc, vc, nq, nkv, d, 0)
+        ops.paged_decode(out, qkv, kc, vc, bt, ctx, to, tm, nq, nkv, 64, 0.09, 100, sinks=3)
+
+    def prompt():
+        ops.prefill_attention(out_p, qkv, kc, vc, bt[:1], cu, ctx[:1], tiles, nq, nkv, 0.09, 100, sinks=3)
+        ops.paged_decode(out, qkv, kc, vc, bt, ctx, to, tm, nq, nkv, 64, 0.09, 0)
+
+    side = torch.cuda.Stream()
+    with torch.cuda.stream(side):
+        graphs = []
+        for work in (decode, prompt):
+            work()
+            side.synchronize()
+            g = torch.cuda.CUDAGraph()
+            with torch.cuda.graph(g, stream=side):
+                work()
+            graphs.append(g)
+        for round_ in range(4):
+            lens = torch.randint(1, width * bs, (b,), generator=gen)
+            lens[0] = max(int(lens[0]), b)
+            table = torch.randperm(nb, generator=gen)[: b * width].view(b, width)
+            fresh = torch.randn(b, n, generator=gen).to(torch.bfloat16)
+            before = kc.clone(), vc.clone()
+            for g, work in zip(graphs, (decode, prompt)):
+                got = []
+                for run in (g.replay, work):
+                    kc.copy_(before[0])
+                    vc.copy_(before[1])
+                    qkv.copy_(fresh)
+                    bt.copy_(table)
+                    ctx.copy_(lens)
+                    pos.copy_(lens - 1)
+                    slots.copy_(table.gather(1, ((lens - 1) // bs)[:, None]).squeeze(1) * bs + (lens - 1) % bs)
+                    to.fill_(float("nan"))
+                    out.fill_(1.0)
+                    run()
+                    side.synchronize()
+                    got.append([x.clone() for x in (out, out_p, kc, vc, qkv)])
+                assert all(torch.equal(a, b_) for a, b_ in zip(*got))
+
+
+# ---------------------------------------------------------------- refusals
+
+@pytest.mark.parametrize("dev", DEVICES)
+def test_refusals(dev):
+    gen = torch.Generator().manual_seed(1)
+    ops, nq, nkv, d, bs = get_ops(dev), 8, 2, 128, 16
+    kc, vc = (c.to(dev) for c in _random_cache(gen, 8, nkv, bs, d))
+    q = _queries(gen, 2, nq, nkv, d).to(dev)
+    out = torch.zeros(2, nq * d, dtype=torch.bfloat16, device=dev)
+    bt, ctx = torch.zeros(2, 4, dtype=torch.int32, device=dev), torch.ones(2, dtype=torch.int32, device=dev)
+    to, tm = torch.zeros(2, nq, 1, d, device=dev), torch.zeros(2, nq, 1, 2, device=dev)
+    cu, tiles = torch.tensor([0, 2], dtype=torch.int32, device=dev), _tiles([2]).to(dev)
+    longs, cs = torch.zeros(2, dtype=torch.long, device=dev), ref.rope_cos_sin(d, 16, 10000.0).to(dev)
+    bad = (ValueError, RuntimeError)
+    for k, v in ((kc[..., :-1], vc), (kc, vc[:4]), (kc, vc.to(torch.int16)), (kc.transpose(0, 1), vc.transpose(0, 1))):
+        with pytest.raises(bad):
+            ops.paged_decode(out, q, k, v, bt, ctx, to, tm, nq, nkv, 64, 0.1)
+        with pytest.raises(bad):
+            ops.prefill_attention(out, q, k, v, bt[:1], cu, ctx[:1], tiles, nq, nkv, 0.1)
+        with pytest.raises(bad):
+            ops.rope_cache(q, longs, longs, cs, k, v, nq, nkv, d, 0)
+        with pytest.raises(bad):
+            ops.read_cache(*(torch.zeros(2, nkv, d, dtype=torch.bfloat16, device=dev) for _ in "kv"), k, v, longs)
+    with pytest.raises(bad):   # other head counts than the cache's
+        ops.paged_decode(out, q, kc, vc, bt, ctx, to, tm, nq, 4, 64, 0.1)
+    with pytest.raises(bad):
+        ops.read_cache(torch.zeros(3, nkv, d, dtype=torch.bfloat16, device=dev), torch.zeros(2, nkv, d, dtype=torch.bfloat16, device=dev), kc, vc,
+                       longs)
+    # first tokens beside a window: the other caches' operators have none
+    kb = torch.zeros(8, nkv, bs, d, dtype=torch.bfloat16, device=dev)
+    vb = torch.zeros(8, nkv, d, bs, dtype=torch.bfloat16, device=dev)
+    with pytest.raises(ValueError):
+        ops.paged_decode(out, q, kb, vb, bt, ctx, to, tm, nq, nkv, 512, 0.1, 16, sinks=4)
+    with pytest.raises(ValueError):
+        ops.prefill_attention(out, q, kb, vb, bt[:1], cu, ctx[:1], tiles, nq, nkv, 0.1, 16, sinks=4)
+
+
+@pytest.mark.gpu
+def test_kernel_refusals():
+    """What only the kernels need: devices, alignment, workspaces, types."""
+    gen = torch.Generator().manual_seed(1)
+    ops, nq, nkv, d, bs = get_ops("cuda"), 8, 2, 128, 16
+    kc, vc = (c.cuda() for c in _random_cache(gen, 8, nkv, bs, d))
+    q = _queries(gen, 2, nq, nkv, d).cuda()
+    n = q.shape[1]
+    out = torch.zeros(2, nq * d, dtype=torch.bfloat16, device="cuda")
+    bt, ctx = torch.zeros(2, 4, dtype=torch.int32, device="cuda"), torch.ones(2, dtype=torch.int32, device="cuda")
+    to, tm = torch.zeros(2, nq, 1, d, device="cuda"), torch.zeros(2, nq, 1, 2, device="cuda")
+    longs, cs = torch.zeros(2, dtype=torch.long, device="cuda"), ref.rope_cos_sin(d, 16, 10000.0).cuda()
+    odd = torch.zeros(2, n + 4, dtype=torch.bfloat16, device="cuda")
+
+    def decode(**kw):
+        a = dict(out=out, q=q, k=kc, v=vc, bt=bt, ctx=ctx, to=to, tm=tm, nq=nq, nkv=nkv, part=64, scale=0.1, window=0, sinks=0)
+        a.update(kw)
+        ops.paged_decode(a["out"], a["q"], a["k"], a["v"], a["bt"], a["ctx"], a["to"], a["tm"], a["nq"], a["nkv"], a["part"], a["scale"],
+                         a["window"], sinks=a["sinks"])
+
+    decode()
+    for kw in (dict(q=q.float()), dict(q=q.cpu()), dict(q=odd[:, :n]), dict(q=odd[:, 4:]), dict(bt=bt.long()), dict(bt=bt.cpu()), dict(ctx=ctx.cpu()),
+               dict(ctx=ctx[:1]), dict(part=96), dict(part=0), dict(part=32768), dict(to=to[:1]), dict(tm=tm.half()), dict(bt=torch.zeros(2, 5, dtype=torch.int32, device="cuda")),
+               dict(window=-1), dict(sinks=-1, window=4), dict(nq=7), dict(out=out[:, :64]), dict(out=out[:1]), dict(v=vc.cpu()), dict(nq=64)):
+        with pytest.raises(RuntimeError):
+            decode(**kw)
+    with pytest.raises(RuntimeError):
+        ops.rope_cache(q, longs[:1], longs, cs, kc, vc, nq, nkv, d, 0)
+    with pytest.raises(RuntimeError):
+        ops.rope_cache(q, longs, longs.int(), cs, kc, vc, nq, nkv, d, 0)
+    with pytest.raises(RuntimeError):
+        ops.rope_cache(q, longs, longs, cs[:, :64], kc, vc, nq, nkv, d, 0)
+    with pytest.raises(RuntimeError):
+        ops.rope_cache(q, longs, longs, cs, kc, vc, nq, nkv, d, 2)
+    with pytest.raises(RuntimeError):
+        ops.rope_cache(q[:, :n - 8], longs, longs, cs, kc, vc, nq, nkv, d, 0)
+    with pytest.raises(RuntimeError):
+        ops.splitk_rope_cache(q, torch.zeros(1, 2, n - 1, device="cuda"), 1, longs, longs, cs, kc, vc, nq, nkv, d, 0)
+    with pytest.raises(RuntimeError):
+        ops.splitk_rope_cache(q, torch.zeros(1, 2, n, device="cuda"), 1, longs, longs, cs, kc, vc, nq, nkv, d, 1, q_w=cs[0], k_w=cs[0])
+
+
+# ---------------------------------------------------------------- the engine
+
+def _model(heads=2, kv_heads=1, dim=64, window=0, layers=2):
+    cfg = PRESETS["tiny-llama"].replace(name="tiny-kv4", hidden_size=heads * dim, num_heads=heads, num_kv_heads=kv_heads, head_dim=dim, num_layers=layers)
+    return cfg.replace(sliding_window=window, layer_windows=(window,) * layers) if window else cfg
+
+
+def _engine(device, mcfg, dtype, **kw):
+    base = dict(model=mcfg.name, load_format="dummy", device=device, dtype=dtype, max_num_seqs=8, max_num_batched_tokens=48, num_kv_blocks=256,
+                max_model_len=512)
+    dev = torch.device("cuda", 0) if device == "cuda" else None
+    return LLMEngine(EngineConfig(**{**base, **kw}), tp=TPGroup(0, 1, None, dev) if dev else TPGroup(), model_cfg=mcfg)
+
+
+def _dense_logits(model, ids, window, sinks):
+    """The whole sequence at once, 32 bits, keys and values rounded to the 4-bit grid, no cache."""
+    cfg = model.cfg
+    x = model.embed[torch.tensor(ids)].float()
+    t, d, nq, nkv = len(ids), cfg.head_dim, cfg.num_heads, cfg.num_kv_heads
+    pos = torch.arange(t)
+    j = pos[None, :]
+    seen = j <= pos[:, None]
+    if window:
+        seen = seen & ((j > pos[:, None] - window) | (j < sinks))
+    for lw in model.layers:
+        h = ref.rmsnorm(x, lw.ln1, cfg.rms_norm_eps)
+        q, k, v = (h @ lw.wqkv.float().T).view(t, -1, d).split((nq, nkv, nkv), 1)
+        q, k = (ref.apply_rope(y, pos, model.cos_sin, cfg.rope_mode) for y in (q, k))
+        k, v = (kv4.dequantise(*kv4.quantise(y.to(torch.bfloat16))).float().repeat_interleave(nq // nkv, 1) for y in (k, v))
+        s = torch.einsum("qhd,khd->hqk", q, k) / math.sqrt(d)
+        o = torch.einsum("hqk,khd->qhd", torch.softmax(s.masked_fill(~seen, float("-inf")), -1), v).reshape(t, nq * d)
+        x = x + o @ lw.wo.float().T
+        gu = ref.rmsnorm(x, lw.ln2, cfg.rms_norm_eps) @ lw.wgu.float().T
+        g, u = gu.chunk(2, -1)
+        x = x + (torch.nn.functional.silu(g) * u) @ lw.wd.float().T
+    return ref.rmsnorm(x, model.norm, cfg.rms_norm_eps)[-1] @ model.lm_head.float().T
+
+
+@pytest.mark.parametrize("window,sinks", [(0, 0), (24, 0), (24, 4)])
+def test_engine_matches_dense(window, sinks):
+    """Chunked prompts and paged decode through the CPU engine against the whole sequence at once."""
+    mcfg = _model(window=window)
+    eng = _engine("cpu", mcfg, "float32", kv_cache_dtype="mxfp4", attention_sinks=sinks)
+    m = eng.runner.model
+    assert eng.runner.kv[0][0].dtype == torch.uint8
+    assert m.kv_bytes_per_block(16) * 32 == 17 * 2 * mcfg.num_layers * mcfg.num_kv_heads * 16 * 64
+    assert sum(c.numel() for kv in eng.runner.kv for c in kv) == m.kv_bytes_per_block(16) * 256
+    prompts = [[1, 5, 9, 33, 70], list(range(3, 100)), list(range(200, 261))]
+    for p, (toks, _, reason) in zip(prompts, eng.generate(prompts, SamplingParams(temperature=0.0, max_tokens=8, ignore_eos=True))):
+        assert reason == "length"
+        ids = list(p)
+        for t in toks:
+            lg = _dense_logits(m, ids, window, sinks)
+            assert lg[t] >= lg.max() - 1e-4
+            ids.append(t)
+
+
+def test_engine_refusals():
+    with pytest.raises(ValueError):
+        EngineConfig(kv_cache_dtype="mxfp4", attention_sinks=-1)
+    with pytest.raises(ValueError):
+        EngineConfig(attention_sinks=4)
+    with pytest.raises(ValueError):
+        EngineConfig(kv_cache_dtype="fp8", attention_sinks=4)
+    with pytest.raises(ValueError):   # heads of 32
+        _engine("cpu", PRESETS["tiny-llama"], "float32", kv_cache_dtype="mxfp4")
+    with pytest.raises(ValueError):   # a design with caches of its own
+        _engine("cpu", PRESETS["tiny-kesirax"], "float32", kv_cache_dtype="mxfp4")
+
+
+def test_command_line():
+    from hipserve.server import cli
+
+    cfg = cli.config_from_args(cli.build_parser().parse_args(["--model", "llama-3-8b", "--kv-cache-dtype", "mxfp4", "--attention-sinks", "4"]))
+    assert cfg.kv_mxfp4 and cfg.attention_sinks == 4
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("window,sinks", [(0, 0), (128, 4)])
+def test_engine_graph_equals_eager(window, sinks):
+    """Llama-3's heads, two layers: captured decode equals eager decode token for token, and the cache takes 17 / 64 of bf16's bytes."""
+    mcfg = PRESETS["llama-3-8b"].replace(name="llama-3-kv4", num_layers=2, hidden_size=1024, intermediate_size=3584, num_heads=8,
+                                         num_kv_heads=2, vocab_size=32000, max_position_embeddings=2048)
+    if window:
+        mcfg = mcfg.replace(sliding_window=window, layer_windows=(window, 0))
+    prompts = [[1] + list(range(100, 400)), [1, 5, 6, 7], list(range(50, 90))]
+    sp = SamplingParams(temperature=0.0, max_tokens=12, ignore_eos=True)
+    toks = {}
+    for kvd, eager in (("mxfp4", False), ("mxfp4", True), ("auto", False)):
+        eng = _engine("cuda", mcfg, "bfloat16", kv_cache_dtype=kvd, attention_sinks=sinks if kvd == "mxfp4" else 0, enforce_eager=eager,
+                      max_num_batched_tokens=256, max_model_len=1024)
+        toks[kvd, eager] = [r[0] for r in eng.generate(prompts, sp)], eng.runner.model.kv_bytes_per_block(16)
+        assert (eng.runner.stats["graph_steps"] > 0) != eager
+        eng.shutdown()
+        del eng
+        torch.cuda.synchronize()
+    assert toks["mxfp4", False] == toks["mxfp4", True]
+    assert toks["mxfp4", False][1] * 64 == toks["auto", False][1] * 17
