@@ -110,11 +110,6 @@ static void kv4_attention(const Kv4Attn& a, const int* cu_q, int seqs, const int
   else kv4_attention_kernel<64><<<grid, 256, 0, s>>>(a, cu_q, seqs, ctx, tiles, rows, o16);
 }
 
-void launch_kv4_decode(const Kv4Attn& a, const int* context_lens, float* tmp_out, float* tmp_ml, int B, int part_size,
-                       int max_parts, void* out16, hipStream_t s) {
-  if (B > 0) kv4_attention(a, nullptr, B, context_lens, nullptr, cdiv(B, 4), B, out16, s);
-}
-
 void launch_kv4_prefill(const Kv4Attn& a, const int* cu_q, int seqs, const int* ctx_lens, int rows, const int* tiles,
                         int ntiles, hipStream_t s) {
   if (ntiles > 0) kv4_attention(a, cu_q, seqs, ctx_lens, tiles, ntiles * 32, rows, nullptr, s);
