@@ -33,6 +33,77 @@ struct Kv4Chunks {
   HS_DEVICE int token(int v) const { return (v < sink ? v : v - sink + first) * kKv4Chunk; }
 };
 
+// Which chunks a workgroup takes. All sequences' chunks are cut into runs of one length, so that ragged batches fill the chip evenly:
+// about kKv4Slots workgroups over the kv heads, what the chip holds at once (two a compute unit). A second round of workgroups costs 6 - 9 us
+// (the chain of lengths, block table and first keys before a wave has work: 64 sequences of 8192 in 512 / 1024 / 2048 workgroups
+// 104 / 113 / 124 us). Every wave works this out for itself from all lengths.
+constexpr int kKv4Slots = 512;
+constexpr int kKv4Waves = 4;  // of a workgroup: 2 and 8 take 1.02 - 1.2 times as long
+
+// sum or maximum (of numbers >= 0) over a wave, and sums up to and with every lane, on the DPP crossbar
+template <int kCtrl, int kRows>
+HS_DEVICE int kv4_dpp(int v) { return __builtin_amdgcn_update_dpp(0, v, kCtrl, kRows, 0xf, false); }
+HS_DEVICE int kv4_scan(int v) {
+  v += kv4_dpp<0x111, 0xf>(v);  // row_shr:1, 2, 4, 8
+  v += kv4_dpp<0x112, 0xf>(v);
+  v += kv4_dpp<0x114, 0xf>(v);
+  v += kv4_dpp<0x118, 0xf>(v);
+  v += kv4_dpp<0x142, 0xa>(v);  // row_bcast:15 -> rows 1, 3
+  v += kv4_dpp<0x143, 0xc>(v);  // row_bcast:31 -> rows 2, 3
+  return v;
+}
+HS_DEVICE int kv4_wave_sum(int v) { return __builtin_amdgcn_readlane(kv4_scan(v), 63); }
+HS_DEVICE int kv4_wave_max(int v) {
+  v = max(v, kv4_dpp<0x111, 0xf>(v));
+  v = max(v, kv4_dpp<0x112, 0xf>(v));
+  v = max(v, kv4_dpp<0x114, 0xf>(v));
+  v = max(v, kv4_dpp<0x118, 0xf>(v));
+  v = max(v, kv4_dpp<0x142, 0xa>(v));
+  v = max(v, kv4_dpp<0x143, 0xc>(v));
+  return __builtin_amdgcn_readlane(v, 63);
+}
+
+struct Kv4Run {
+  int chunks;        // of a run
+  int b, part, ctx;  // the workgroup's sequence (B: it has none), its partition, the sequence's length
+};
+
+HS_DEVICE int kv4_length(const int* __restrict__ ctx_lens, int B, int b, int cap) { return b < B ? min(ctx_lens[b], cap) : 0; }
+
+// `own` >= 0: of that sequence; else of workgroup w among the runs of all sequences, where one without keys has one run
+HS_DEVICE Kv4Run kv4_run(const int* __restrict__ ctx_lens, int B, int cap, int window, int sinks, int nkv, int max_parts,
+                         int own, int w) {
+  const int lane = threadIdx.x & 63;
+  const int len0 = kv4_length(ctx_lens, B, lane, cap);
+  int total = Kv4Chunks(len0, window, sinks).count, most = total;
+  for (int b = 64 + lane; b < B; b += 64) {
+    const int n = Kv4Chunks(kv4_length(ctx_lens, B, b, cap), window, sinks).count;
+    total += n;
+    most = max(most, n);
+  }
+  total = kv4_wave_sum(total);
+  most = kv4_wave_max(most);
+  // a sequence's last run is half a run short on average. The quotient in 32-bit floats, and one more: never below the true one by
+  // what the grid does not cover
+  const int slots = max(kKv4Slots - B * nkv / 2, kKv4Slots / 2);
+  int run = max((int)((float)total * (float)nkv / (float)slots) + 1, (most + max_parts - 1) / max_parts);
+  run = (run + kKv4Waves - 1) / kKv4Waves * kKv4Waves;
+  if (own >= 0) return {run, own, 0, kv4_length(ctx_lens, B, own, cap)};
+  int before = 0;
+  for (int b0 = 0; b0 < B; b0 += 64) {
+    const int len = b0 == 0 ? len0 : kv4_length(ctx_lens, B, b0 + lane, cap);
+    const int n = b0 + lane < B ? max((Kv4Chunks(len, window, sinks).count + run - 1) / run, 1) : 0;
+    const int upto = before + kv4_scan(n);
+    const unsigned long after = __ballot(upto > w);
+    if (after) {
+      const int l = __builtin_ctzl(after);
+      return {run, b0 + l, w - __builtin_amdgcn_readlane(upto - n, l), __builtin_amdgcn_readlane(len, l)};
+    }
+    before = __builtin_amdgcn_readlane(upto, 63);
+  }
+  return {run, B, 0, 0};
+}
+
 // 16 values as e4m3 numbers hi + lo / 16
 HS_DEVICE void kv4_split16(const float (&x)[16], u32x4& hi, u32x4& lo) {
 #pragma unroll
@@ -67,19 +138,24 @@ HS_DEVICE unsigned kv4_keep_scales(unsigned w, unsigned keep) {
   return (w & m) | (0x7f7f7f7fu & ~m);
 }
 
-template <int D, int W>
-__global__ __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu(2, 8))) void kv4_decode_kernel(Kv4Attn a, const int* __restrict__ ctx_lens,
+template <int D>
+__global__ __launch_bounds__(64 * kKv4Waves) __attribute__((amdgpu_waves_per_eu(2, 8))) void kv4_decode_kernel(Kv4Attn a, const int* __restrict__ ctx_lens,
                                                             float* __restrict__ tmp_out, float* __restrict__ tmp_ml,
-                                                            int part_chunks, int max_parts,
-                                                            unsigned short* __restrict__ out16) {
+                                                            int B, int max_parts, unsigned short* __restrict__ out16) {
   constexpr int NG = D / 32;             // scale groups of a head
+  constexpr int W = kKv4Waves;
   constexpr int NK = D == 64 ? 2 : 4;    // K loads a chunk: at 64 dims the upper lanes of a product take other tokens
-  const int part = blockIdx.x, kh = blockIdx.y, b = blockIdx.z;
+  const int kh = blockIdx.y;
   const int nq = a.nq, nkv = a.cache.nkv, bs = a.cache.block_size, G = nq / nkv;
-  const int ctx = min(ctx_lens[b], a.bt_width * bs);
+  const int cap = a.bt_width * bs;
+  Kv4Run run{INT32_MAX / kKv4Chunk, (int)blockIdx.x, 0, 0};
+  if (max_parts > 1) run = kv4_run(ctx_lens, B, cap, a.window, a.sinks, nkv, max_parts, -1, blockIdx.x);
+  else run.ctx = min(ctx_lens[run.b], cap);
+  if (run.b >= B) return;
+  const int b = run.b, part = run.part, part_chunks = run.chunks, ctx = run.ctx;
   const Kv4Chunks chunks(ctx, a.window, a.sinks);
   const int c0 = part * part_chunks, c1 = min(c0 + part_chunks, chunks.count);
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   unsigned short* out = static_cast<unsigned short*>(a.out) + (long)b * a.out_stride + (long)kh * G * D;
   if (c0 >= c1) {
     if (part == 0)  // a row without keys
@@ -94,14 +170,8 @@ __global__ __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu(2, 8))) 
   extern __shared__ __attribute__((aligned(16))) char smem[];
   float* olds = reinterpret_cast<float*>(smem);              // [W][G][D]
   float* red = olds + W * G * D;                             // [W][G][2]
-  int* pages = reinterpret_cast<int*>(red + W * G * 2);      // 4 a chunk: a run of 16 tokens lies in one page
   const int* bt = a.block_tables + (long)b * a.bt_stride;
   const int bsh = __builtin_ctz(bs), bmask = bs - 1;
-  for (int i = tid; i < (c1 - c0) * 4; i += 64 * W) {
-    const int tok = chunks.token(c0 + (i >> 2)) + 16 * (i & 3);
-    pages[i] = tok < ctx ? kv4_page(bt[tok >> bsh], a.cache.blocks) : -1;
-  }
-  __syncthreads();
 
   // ---- loads of a chunk
   const long head_bytes = kv4_head_bytes(bs, D), page_bytes = head_bytes * nkv;
@@ -116,10 +186,18 @@ __global__ __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu(2, 8))) 
     unsigned ks;
     int page;  // of this lane's 16 tokens
   };
-  auto load = [&](int c, Chunk& ch) {
-    c = min(c, c1 - 1);
-    const int tok = chunks.token(c);
-    const int kp = pages[(c - c0) * 4 + (col >> 2)], vp = pages[(c - c0) * 4 + grp];
+  // a run of 16 tokens lies in one page: the pages of a lane's keys and values. They are asked for a chunk before its loads, and
+  // before the loads of the chunk between, so that the wait for them is for nothing younger
+  struct Pages {
+    int k, v;
+  };
+  auto pages = [&](int c) {
+    const int tok = chunks.token(min(c, c1 - 1));
+    return Pages{bt[min(tok + 16 * (col >> 2), ctx - 1) >> bsh], bt[min(tok + 16 * grp, ctx - 1) >> bsh]};
+  };
+  auto load = [&](int c, const Pages& pg, Chunk& ch) {
+    const int tok = chunks.token(min(c, c1 - 1));
+    const int kp = kv4_page(pg.k, a.cache.blocks), vp = kv4_page(pg.v, a.cache.blocks);
     const int ko = (tok + 16 * (col >> 2)) & bmask, vo = (tok + 16 * grp) & bmask;
     const unsigned char* k = kbase + (long)max(kp, 0) * page_bytes;
     const unsigned char* kc = k + (ko + krow) * (D / 2) + 16 * kgrp;
@@ -136,14 +214,11 @@ __global__ __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu(2, 8))) 
     ch.page = vp;
   };
 
-  // ---- q: head `col`, dims 16 grp .. and 64 + 16 grp .. of the product's k
-  i32x8 qhi[D == 64 ? 2 : 1], qlo[D == 64 ? 2 : 1];
-  float sl;
+  // ---- q: head `col`, dims 16 grp .. and 64 + 16 grp .. of the product's k; on its way before the first chunk
+  constexpr int NH = D == 64 ? 1 : 2;
+  u16x8 raw[NH][2];
   {
     const unsigned short* qp = static_cast<const unsigned short*>(a.q) + (long)b * a.q_stride + (long)(kh * G + col) * D;
-    constexpr int NH = D == 64 ? 1 : 2;
-    u16x8 raw[NH][2];
-    unsigned am = 0;
 #pragma unroll
     for (int h = 0; h < NH; ++h)
 #pragma unroll
@@ -151,8 +226,26 @@ __global__ __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu(2, 8))) 
         const int d0 = 64 * h + 16 * grp + 8 * e;
         raw[h][e] = u16x8{0, 0, 0, 0, 0, 0, 0, 0};
         if (col < G && d0 < D) raw[h][e] = *reinterpret_cast<const u16x8*>(qp + d0);
-        am = max(am, kv4_amax8(raw[h][e]));
       }
+  }
+  Chunk A, B_;
+  Pages pg;
+  const int c = c0 + wave;
+  if (c < c1) {
+    pg = pages(c);
+    const Pages next = pages(c + W);
+    load(c, pg, A);
+    pg = next;
+  }
+  i32x8 qhi[D == 64 ? 2 : 1], qlo[D == 64 ? 2 : 1];
+  float sl;
+  {
+    unsigned am = 0;
+#pragma unroll
+    for (int h = 0; h < NH; ++h)
+#pragma unroll
+      for (int e = 0; e < 2; ++e)
+        am = max(am, kv4_amax8(raw[h][e]));
     am = max(am, (unsigned)__shfl_xor((int)am, 16, 64));
     am = max(am, (unsigned)__shfl_xor((int)am, 32, 64));
     const int eb = min(max((int)(am >> 7), 8), 254);  // the largest value comes to [128, 256)
@@ -185,7 +278,7 @@ __global__ __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu(2, 8))) 
   for (int n = 0; n < NG; ++n) o[n][0] = o[n][1] = f32x4{0.f, 0.f, 0.f, 0.f};
   float m_run = -1e30f, l_run = 0.f;  // of head `col`; the sum over this lane's tokens alone
 
-  auto compute = [&](int c, const Chunk& ch) {
+  auto compute = [&](int c, Chunk& ch) {
     const int tok = chunks.token(c);
     // ---- scores of tokens tok + 16 grp + 4 t + r for head `col`
     f32x4 st[4];
@@ -203,19 +296,18 @@ __global__ __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu(2, 8))) 
       st[2] = kv4_scores<2>(ch.k[2], ks, qhi[0], qlo[0]);
       st[3] = kv4_scores<3>(ch.k[3], ks, qhi[0], qlo[0]);
     }
-    unsigned vis = 0xffffu;  // which of this lane's 16 tokens are visible
     const bool whole = tok + kKv4Chunk <= ctx && (tok >= chunks.lo || tok + kKv4Chunk <= a.sinks);
-    const bool edge = !whole || __any(ch.page < 0);
-    if (edge) {
-      vis = 0;
+    if (!whole || __any(ch.page < 0)) {
+      // which of this lane's 16 tokens are visible, as bits: below ctx, and in the window or among the sinks
+      const int j0 = tok + 16 * grp;
+      auto below = [](int n) { return n <= 0 ? 0u : n >= 16 ? 0xffffu : (1u << n) - 1u; };
+      const unsigned vis = ch.page < 0 ? 0u : below(ctx - j0) & (~below(chunks.lo - j0) | below(a.sinks - j0));
 #pragma unroll
-      for (int i = 0; i < 16; ++i) {
-        const int j = tok + 16 * grp + i;
-        if (ch.page >= 0 && j < ctx && (j >= chunks.lo || j < a.sinks)) vis |= 1u << i;
-      }
+      for (int i = 0; i < 16; ++i) st[i >> 2][i & 3] = vis >> i & 1 ? st[i >> 2][i & 3] : -INFINITY;
 #pragma unroll
-      for (int i = 0; i < 16; ++i)
-        if (!(vis >> i & 1)) st[i >> 2][i & 3] = -INFINITY;
+      for (int n = 0; n < NG; ++n)
+#pragma unroll
+        for (int q = 0; q < 4; ++q) ch.vs[n][q] = kv4_keep_scales(ch.vs[n][q], vis >> (4 * q));
     }
     float mx = -INFINITY;
 #pragma unroll
@@ -254,8 +346,7 @@ __global__ __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu(2, 8))) 
 #pragma unroll
       for (int q = 0; q < 4; ++q) {  // tokens 4 q .. 4 q + 3 of the lane's 16
         const unsigned w = ch.v[n][q];
-        unsigned s = ch.vs[n][q];
-        if (edge) s = kv4_keep_scales(s, vis >> (4 * q));
+        const unsigned s = ch.vs[n][q];
         const unsigned x0 = kv4_widen2<0>(w, __uint_as_float(s << 23)), x1 = kv4_widen2<1>(w, __uint_as_float(s << 15));
         const unsigned x2 = kv4_widen2<2>(w, __uint_as_float(s << 7)), x3 = kv4_widen2<3>(w, __uint_as_float(s >> 1));
         even[q >> 1][2 * (q & 1)] = __builtin_amdgcn_perm(x1, x0, 0x05040100u);
@@ -271,19 +362,21 @@ __global__ __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu(2, 8))) 
     }
   };
 
-  Chunk A, B;
-  int c = c0 + wave;
   if (c < c1) {
-    load(c, A);
-    for (; c + W < c1; c += 2 * W) {
-      load(c + W, B);
+    int i = c;
+    for (; i + W < c1; i += 2 * W) {
+      Pages next = pages(i + 2 * W);
+      load(i + W, pg, B_);
+      pg = next;
       __builtin_amdgcn_sched_barrier(0);
-      compute(c, A);
-      load(c + 2 * W, A);
+      compute(i, A);
+      next = pages(i + 3 * W);
+      load(i + 2 * W, pg, A);
+      pg = next;
       __builtin_amdgcn_sched_barrier(0);
-      compute(c + W, B);
+      compute(i + W, B_);
     }
-    if (c < c1) compute(c, A);
+    if (i < c1) compute(i, A);
   }
 
   // ---- the waves' results
@@ -330,67 +423,77 @@ __global__ __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu(2, 8))) 
   }
 }
 
-// Merges a row's partitions: a workgroup per (head, sequence), lane groups of D lanes take every kGroups-th partition, four at a time.
+// Merges a row's partitions: a workgroup per (head, sequence), D / 4 lanes of four dims a partition, four partitions of a lane at a
+// time. Few waves, as rows of one partition have nothing to merge: 2048 workgroups of 16 waves that only found that out took 9 us.
 template <int D>
-__global__ __launch_bounds__(384) void kv4_decode_merge_kernel(Kv4Attn a, const int* __restrict__ ctx_lens,
+__global__ __launch_bounds__(256) void kv4_decode_merge_kernel(Kv4Attn a, const int* __restrict__ ctx_lens,
                                                                const float* __restrict__ tmp_out,
-                                                               const float* __restrict__ tmp_ml, int part_chunks,
-                                                               int max_parts, unsigned short* __restrict__ out16) {
-  constexpr int kGroups = 384 / D;
-  const int h = blockIdx.x, b = blockIdx.y, tid = threadIdx.x, d = tid % D, grp = tid / D;
-  const Kv4Chunks chunks(min(ctx_lens[b], a.bt_width * a.cache.block_size), a.window, a.sinks);
-  if (chunks.count <= part_chunks) return;
-  const int np = (chunks.count + part_chunks - 1) / part_chunks;
+                                                               const float* __restrict__ tmp_ml, int B, int max_parts,
+                                                               unsigned short* __restrict__ out16) {
+  constexpr int kLanes = D / 4, kGroups = 256 / kLanes;
+  const int h = blockIdx.x, b = blockIdx.y, tid = threadIdx.x, d4 = tid % kLanes, grp = tid / kLanes;
+  const Kv4Run run = kv4_run(ctx_lens, B, a.bt_width * a.cache.block_size, a.window, a.sinks, a.cache.nkv, max_parts, b, 0);
+  const int count = Kv4Chunks(run.ctx, a.window, a.sinks).count;
+  if (count <= run.chunks) return;
+  const int np = (count + run.chunks - 1) / run.chunks;
   const long base = ((long)b * a.nq + h) * max_parts;
   float M = -1e30f;
   for (int p = tid & 63; p < np; p += 64) M = fmaxf(M, tmp_ml[(base + p) * 2]);
   M = wave_max(M);
-  float L[4] = {0.f, 0.f, 0.f, 0.f}, acc[4] = {0.f, 0.f, 0.f, 0.f};
-  for (int p = grp; p < np; p += 4 * kGroups)
+  float L[4] = {0.f, 0.f, 0.f, 0.f};
+  f32x4 acc[4];
 #pragma unroll
-    for (int u = 0; u < 4; ++u) {
-      const long q = base + min(p + u * kGroups, np - 1);
-      const float w = __builtin_amdgcn_exp2f(tmp_ml[q * 2] - M) * tmp_ml[q * 2 + 1], x = tmp_out[q * D + d];
-      if (p + u * kGroups < np) {
-        L[u] += w;
-        acc[u] += w * x;
+  for (int u = 0; u < 4; ++u) acc[u] = f32x4{0.f, 0.f, 0.f, 0.f};
+  if (grp < kGroups)
+    for (int p = grp; p < np; p += 4 * kGroups)
+#pragma unroll
+      for (int u = 0; u < 4; ++u) {
+        const long q = base + min(p + u * kGroups, np - 1);
+        const float w = __builtin_amdgcn_exp2f(tmp_ml[q * 2] - M) * tmp_ml[q * 2 + 1];
+        const f32x4 x = *reinterpret_cast<const f32x4*>(tmp_out + q * D + 4 * d4);
+        if (p + u * kGroups < np) {
+          L[u] += w;
+          acc[u] += w * x;
+        }
       }
-    }
-  __shared__ float sums[2][kGroups][D];
-  sums[0][grp][d] = (L[0] + L[1]) + (L[2] + L[3]);
-  sums[1][grp][d] = (acc[0] + acc[1]) + (acc[2] + acc[3]);
+  __shared__ f32x4 sums[kGroups][kLanes];
+  __shared__ float ls[kGroups];
+  if (grp < kGroups) {
+    sums[grp][d4] = (acc[0] + acc[1]) + (acc[2] + acc[3]);
+    if (d4 == 0) ls[grp] = (L[0] + L[1]) + (L[2] + L[3]);
+  }
   __syncthreads();
-  if (grp == 0) {
+  if (tid < D) {
     float l = 0.f, y = 0.f;
 #pragma unroll
     for (int g = 0; g < kGroups; ++g) {
-      l += sums[0][g][d];
-      y += sums[1][g][d];
+      l += ls[g];
+      y += sums[g][tid >> 2][tid & 3];
     }
     const unsigned short ob = f32_to_bf16(l == 0.f ? 0.f : y / l);
-    static_cast<unsigned short*>(a.out)[(long)b * a.out_stride + (long)h * D + d] = ob;
-    if (out16 != nullptr) store_o16(out16, (long)b * a.out_stride, h * D + d, ob);
+    static_cast<unsigned short*>(a.out)[(long)b * a.out_stride + (long)h * D + tid] = ob;
+    if (out16 != nullptr) store_o16(out16, (long)b * a.out_stride, h * D + tid, ob);
   }
 }
 
 template <int D>
-static void kv4_decode(const Kv4Attn& a, const int* ctx, float* tmp_out, float* tmp_ml, int B, int part_size, int max_parts,
+static void kv4_decode(const Kv4Attn& a, const int* ctx, float* tmp_out, float* tmp_ml, int B, int max_parts,
                        unsigned short* out16, hipStream_t s) {
-  const int G = a.nq / a.cache.nkv, chunks = part_size / kKv4Chunk;
-  const dim3 grid(max_parts, a.cache.nkv, B);
-  auto smem = [&](int w) { return (size_t)w * G * (D + 2) * sizeof(float) + (size_t)chunks * 4 * sizeof(int); };
-  kv4_decode_kernel<D, 4><<<grid, 256, smem(4), s>>>(a, ctx, tmp_out, tmp_ml, chunks, max_parts, out16);
-  if (max_parts > 1)
-    kv4_decode_merge_kernel<D><<<dim3(a.nq, B), 384, 0, s>>>(a, ctx, tmp_out, tmp_ml, chunks, max_parts, out16);
+  const int nkv = a.cache.nkv, G = a.nq / nkv;
+  // one partition: a workgroup per sequence and kv head; else the runs of kv4_run, at most so many and one more a sequence
+  const dim3 grid(max_parts > 1 ? cdiv(kKv4Slots, nkv) + B : B, nkv);
+  const size_t smem = (size_t)kKv4Waves * G * (D + 2) * sizeof(float);
+  kv4_decode_kernel<D><<<grid, 64 * kKv4Waves, smem, s>>>(a, ctx, tmp_out, tmp_ml, B, max_parts, out16);
+  if (max_parts > 1) kv4_decode_merge_kernel<D><<<dim3(a.nq, B), 256, 0, s>>>(a, ctx, tmp_out, tmp_ml, B, max_parts, out16);
 }
 
 void launch_kv4_decode(const Kv4Attn& a, const int* context_lens, float* tmp_out, float* tmp_ml, int B, int part_size,
                        int max_parts, void* out16, hipStream_t s) {
   if (B <= 0) return;
   auto* o16 = static_cast<unsigned short*>(out16);
-  if (a.cache.D == 128) kv4_decode<128>(a, context_lens, tmp_out, tmp_ml, B, part_size, max_parts, o16, s);
-  else if (a.cache.D == 96) kv4_decode<96>(a, context_lens, tmp_out, tmp_ml, B, part_size, max_parts, o16, s);
-  else kv4_decode<64>(a, context_lens, tmp_out, tmp_ml, B, part_size, max_parts, o16, s);
+  if (a.cache.D == 128) kv4_decode<128>(a, context_lens, tmp_out, tmp_ml, B, max_parts, o16, s);
+  else if (a.cache.D == 96) kv4_decode<96>(a, context_lens, tmp_out, tmp_ml, B, max_parts, o16, s);
+  else kv4_decode<64>(a, context_lens, tmp_out, tmp_ml, B, max_parts, o16, s);
 }
 
 }  // namespace hipserve
