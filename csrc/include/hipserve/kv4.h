@@ -63,6 +63,28 @@ HS_DEVICE unsigned kv4_widen2(unsigned w, float s) {
   return __builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, s, kByte));
 }
 
+// 8 bf16 values over scale (its exponent) as e4m3 numbers hi + lo / 16: the upper four of their eight significant bits, and the rest
+HS_DEVICE void kv4_split8(const u16x8 v, float scale, float scale16, u32x2& hi, u32x2& lo) {
+  typedef short i16x2 __attribute__((ext_vector_type(2)));
+#pragma unroll
+  for (int w = 0; w < 2; ++w) {
+    float h[4], l[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const float x = bf16_to_f32(v[4 * w + j]);
+      h[j] = __uint_as_float(__float_as_uint(x) & 0xfff00000u);
+      l[j] = x - h[j];
+    }
+    i16x2 hp = {0, 0}, lp = {0, 0};
+    hp = __builtin_amdgcn_cvt_scalef32_pk_fp8_f32(hp, h[0], h[1], scale, false);
+    hp = __builtin_amdgcn_cvt_scalef32_pk_fp8_f32(hp, h[2], h[3], scale, true);
+    lp = __builtin_amdgcn_cvt_scalef32_pk_fp8_f32(lp, l[0], l[1], scale16, false);
+    lp = __builtin_amdgcn_cvt_scalef32_pk_fp8_f32(lp, l[2], l[3], scale16, true);
+    hi[w] = __builtin_bit_cast(unsigned, hp);
+    lo[w] = __builtin_bit_cast(unsigned, lp);
+  }
+}
+
 // Blocks' ids of a sequence come from its block table. One outside of the cache is no page: its keys are not visible.
 HS_DEVICE int kv4_page(int id, long blocks) { return (unsigned)id < (unsigned long)blocks ? id : -1; }
 

@@ -104,22 +104,6 @@ HS_DEVICE Kv4Run kv4_run(const int* __restrict__ ctx_lens, int B, int cap, int w
   return {run, B, 0, 0};
 }
 
-// 16 values as e4m3 numbers hi + lo / 16
-HS_DEVICE void kv4_split16(const float (&x)[16], u32x4& hi, u32x4& lo) {
-#pragma unroll
-  for (int w = 0; w < 4; ++w) {
-    int h = 0, l = 0;
-    h = __builtin_amdgcn_cvt_pk_fp8_f32(x[4 * w], x[4 * w + 1], h, false);
-    h = __builtin_amdgcn_cvt_pk_fp8_f32(x[4 * w + 2], x[4 * w + 3], h, true);
-    const float r0 = x[4 * w] - __builtin_amdgcn_cvt_f32_fp8(h, 0), r1 = x[4 * w + 1] - __builtin_amdgcn_cvt_f32_fp8(h, 1);
-    const float r2 = x[4 * w + 2] - __builtin_amdgcn_cvt_f32_fp8(h, 2), r3 = x[4 * w + 3] - __builtin_amdgcn_cvt_f32_fp8(h, 3);
-    l = __builtin_amdgcn_cvt_pk_fp8_f32(r0 * 16.f, r1 * 16.f, l, false);
-    l = __builtin_amdgcn_cvt_pk_fp8_f32(r2 * 16.f, r3 * 16.f, l, true);
-    hi[w] = (unsigned)h;
-    lo[w] = (unsigned)l;
-  }
-}
-
 HS_DEVICE i32x8 kv4_pad(const u32x4 a, const u32x4 b) {
   return i32x8{(int)a[0], (int)a[1], (int)a[2], (int)a[3], (int)b[0], (int)b[1], (int)b[2], (int)b[3]};
 }
@@ -248,19 +232,22 @@ __global__ __launch_bounds__(64 * kKv4Waves) __attribute__((amdgpu_waves_per_eu(
         am = max(am, kv4_amax8(raw[h][e]));
     am = max(am, (unsigned)__shfl_xor((int)am, 16, 64));
     am = max(am, (unsigned)__shfl_xor((int)am, 32, 64));
-    const int eb = min(max((int)(am >> 7), 8), 254);  // the largest value comes to [128, 256)
-    float up = __uint_as_float((unsigned)(261 - eb) << 23);
-    if (a.scale < 0.f) up = -up;  // the multiplier below is not negative: the largest product has the largest score
+    const int eb = min(max((int)(am >> 7), 16), 254);  // the largest value comes to [128, 256)
+    const float down = __uint_as_float((unsigned)(eb - 7) << 23), down16 = __uint_as_float((unsigned)(eb - 11) << 23);
     // never 0: a hidden key's -inf has to stay one
-    sl = am >= 0x7f80u ? NAN : fmaxf(fabsf(a.scale) * kLog2E * __uint_as_float((unsigned)(eb - 7) << 23), 1.17549435e-38f);
+    sl = am >= 0x7f80u ? NAN : fmaxf(a.scale * kLog2E * down, 1.17549435e-38f);
     u32x4 hi[NH], lo[NH];
 #pragma unroll
-    for (int h = 0; h < NH; ++h) {
-      float x[16];
+    for (int h = 0; h < NH; ++h)
 #pragma unroll
-      for (int j = 0; j < 16; ++j) x[j] = am >= 0x7f80u ? 0.f : bf16_to_f32(raw[h][j >> 3][j & 7]) * up;
-      kv4_split16(x, hi[h], lo[h]);
-    }
+      for (int e = 0; e < 2; ++e) {
+        u32x2 x, y;
+        kv4_split8(raw[h][e], down, down16, x, y);
+        hi[h][2 * e] = x[0];
+        hi[h][2 * e + 1] = x[1];
+        lo[h][2 * e] = y[0];
+        lo[h][2 * e + 1] = y[1];
+      }
     const u32x4 z{0, 0, 0, 0};
     if constexpr (D == 64) {
       qhi[0] = kv4_pad(hi[0], z);

@@ -30,22 +30,6 @@ HS_DEVICE float kv4_sum32(float v) {
   return __builtin_bit_cast(float, (unsigned)r[0]) + __builtin_bit_cast(float, (unsigned)r[1]);
 }
 
-// 8 values as e4m3 numbers hi + lo / 16
-HS_DEVICE void kv4_split8(const float (&x)[8], u32x2& hi, u32x2& lo) {
-#pragma unroll
-  for (int w = 0; w < 2; ++w) {
-    int h = 0, l = 0;
-    h = __builtin_amdgcn_cvt_pk_fp8_f32(x[4 * w], x[4 * w + 1], h, false);
-    h = __builtin_amdgcn_cvt_pk_fp8_f32(x[4 * w + 2], x[4 * w + 3], h, true);
-    const float r0 = x[4 * w] - __builtin_amdgcn_cvt_f32_fp8(h, 0), r1 = x[4 * w + 1] - __builtin_amdgcn_cvt_f32_fp8(h, 1);
-    const float r2 = x[4 * w + 2] - __builtin_amdgcn_cvt_f32_fp8(h, 2), r3 = x[4 * w + 3] - __builtin_amdgcn_cvt_f32_fp8(h, 3);
-    l = __builtin_amdgcn_cvt_pk_fp8_f32(r0 * 16.f, r1 * 16.f, l, false);
-    l = __builtin_amdgcn_cvt_pk_fp8_f32(r2 * 16.f, r3 * 16.f, l, true);
-    hi[w] = (unsigned)h;
-    lo[w] = (unsigned)l;
-  }
-}
-
 // whether a byte of w is 255
 HS_DEVICE bool kv4_any_nan(unsigned w) { return (((w & 0x7f7f7f7fu) + 0x01010101u) & w & 0x80808080u) != 0; }
 HS_DEVICE unsigned kv4_no_nan(unsigned w) {  // 255 -> 127
@@ -209,20 +193,16 @@ __global__ __launch_bounds__(64 * NWV) __attribute__((amdgpu_waves_per_eu(2, 8))
         am = max(am, kv4_amax8(raw[s][e]));
       }
     am = max(am, (unsigned)__shfl_xor((int)am, 32, 64));
-    const int eb = min(max((int)(am >> 7), 8), 254);  // the largest value comes to [128, 256)
-    float up = __uint_as_float((unsigned)(261 - eb) << 23);
-    if (a.scale < 0.f) up = -up;
+    const int eb = min(max((int)(am >> 7), 16), 254);  // the largest value comes to [128, 256)
+    const float down = __uint_as_float((unsigned)(eb - 7) << 23), down16 = __uint_as_float((unsigned)(eb - 11) << 23);
     // never 0: a hidden key's -inf has to stay one
-    sl = am >= 0x7f80u ? NAN : fmaxf(fabsf(a.scale) * kLog2E * __uint_as_float((unsigned)(eb - 7) << 23), 1.17549435e-38f);
+    sl = am >= 0x7f80u ? NAN : fmaxf(a.scale * kLog2E * down, 1.17549435e-38f);
 #pragma unroll
     for (int s = 0; s < KS; ++s)
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
-        float x[8];
-#pragma unroll
-        for (int j = 0; j < 8; ++j) x[j] = am >= 0x7f80u ? 0.f : bf16_to_f32(raw[s][e][j]) * up;
         u32x2 hi, lo2;
-        kv4_split8(x, hi, lo2);
+        kv4_split8(raw[s][e], down, down16, hi, lo2);
         qhi[s][2 * e] = (int)hi[0];
         qhi[s][2 * e + 1] = (int)hi[1];
         qlo[s][2 * e] = (int)lo2[0];
@@ -273,15 +253,29 @@ __global__ __launch_bounds__(64 * NWV) __attribute__((amdgpu_waves_per_eu(2, 8))
                        (window <= 0 || key > wmax - window || key + kKv4Tile <= sinks) && gone == 0;
     if (!whole) {
       const int lim = min(pos, cap - 1) - key - 8 * half;  // offsets above: behind the row
-      const int wlo = window > 0 ? pos - window - key - 8 * half : -kKv4Tile;  // offsets up to this one: before the window
-      const int slo = sinks - key - 8 * half;                                 // unless below this one
+      if (window <= 0) {
 #pragma unroll
-      for (int h2 = 0; h2 < 2; ++h2)
+        for (int h2 = 0; h2 < 2; ++h2)
 #pragma unroll
-        for (int r = 0; r < 16; ++r) {
-          const int off = 32 * h2 + 16 * (r >> 3) + (r & 7);
-          if (off > lim || (off <= wlo && off >= slo) || (gone >> (8 * (2 * h2 + (r >> 3))) & 255u)) st[h2][r] = -INFINITY;
-        }
+          for (int r = 0; r < 16; ++r) st[h2][r] = 32 * h2 + 16 * (r >> 3) + (r & 7) > lim ? -INFINITY : st[h2][r];
+      } else {
+        const int wlo = pos - window - key - 8 * half;  // offsets up to this one: before the window,
+        const int slo = sinks - key - 8 * half;         // and hidden unless below this one
+#pragma unroll
+        for (int h2 = 0; h2 < 2; ++h2)
+#pragma unroll
+          for (int r = 0; r < 16; ++r) {
+            const int off = 32 * h2 + 16 * (r >> 3) + (r & 7);
+            const bool hidden = (off > lim) | ((off <= wlo) & (off >= slo));
+            st[h2][r] = hidden ? -INFINITY : st[h2][r];
+          }
+      }
+      if (gone)
+#pragma unroll
+        for (int h2 = 0; h2 < 2; ++h2)
+#pragma unroll
+          for (int r = 0; r < 16; ++r)
+            if (gone >> (8 * (2 * h2 + (r >> 3))) & 255u) st[h2][r] = -INFINITY;
     }
     float mx = -INFINITY;
 #pragma unroll

@@ -339,6 +339,7 @@ static hipserve::Kv4Attn kv4_attn(at::Tensor& out, const at::Tensor& q, const at
   a.cache = kv4_cache(k_cache, v_cache, nkv, who);
   TORCH_CHECK(nq > 0 && nq % nkv == 0 && nq / nkv <= 16 && nq < 65536, who, ": nq a multiple of nkv, at most 16 queries per kv head");
   TORCH_CHECK(window >= 0 && sinks >= 0 && window <= INT32_MAX && sinks <= INT32_MAX, who, ": window >= 0, sinks >= 0");
+  TORCH_CHECK(scale >= 0, who, ": scale >= 0");
   kv4_rows(q, k_cache, nq * a.cache.D, who, "q");
   kv4_rows(out, k_cache, nq * a.cache.D, who, "out");
   TORCH_CHECK(block_tables.device() == k_cache.device() && block_tables.scalar_type() == at::kInt && block_tables.dim() == 2 &&

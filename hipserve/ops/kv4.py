@@ -124,6 +124,8 @@ def context(k_cache, v_cache, block_table, n: int):
 def attend(q, k, v, seen, scale: float) -> torch.Tensor:
     """q [rows, heads, D], k and v [n, kv heads, D], seen [rows, n] -> [rows, heads, D]: softmax over what is seen, zeros for a row that
     sees nothing. What a hidden key or value holds, NaN or not, never enters."""
+    if not scale >= 0:
+        raise ValueError(f"scale >= 0, got {scale}")
     rows, nq, D = q.shape
     g = nq // k.shape[1]
     q = q.float().unflatten(1, (-1, g)).transpose(0, 1)                   # [kv heads, rows, g, D]

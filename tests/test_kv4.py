@@ -613,6 +613,11 @@ def test_refusals(dev):
             ops.read_cache(*(torch.zeros(2, nkv, d, dtype=torch.bfloat16, device=dev) for _ in "kv"), k, v, longs)
     with pytest.raises(bad):   # other head counts than the cache's
         ops.paged_decode(out, q, kc, vc, bt, ctx, to, tm, nq, 4, 64, 0.1)
+    for scale in (-0.1, float("nan")):
+        with pytest.raises(bad):
+            ops.paged_decode(out, q, kc, vc, bt, ctx, to, tm, nq, nkv, 64, scale)
+        with pytest.raises(bad):
+            ops.prefill_attention(out, q, kc, vc, bt[:1], cu, ctx[:1], tiles, nq, nkv, scale)
     with pytest.raises(bad):
         ops.read_cache(torch.zeros(3, nkv, d, dtype=torch.bfloat16, device=dev), torch.zeros(2, nkv, d, dtype=torch.bfloat16, device=dev), kc, vc,
                        longs)
