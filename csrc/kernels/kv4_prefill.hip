@@ -2,8 +2,10 @@
 // that stay visible beside it. Keys of the step itself come from the cache like the older ones: kv4_write has run before.
 //
 // Bound by the matrix cores and by what stands beside their products, so a tile is unpacked once for all its readers:
-//  * workgroup = up to 8 query heads of one kv head x blocks of 32 rows, a wave each; 64 keys a tile, two LDS buffers, one barrier
-//    a tile, the loads of the next two tiles in registers.
+//  * workgroup = up to 8 query heads of one kv head x blocks of 32 rows, a wave each; 64 keys a tile, staged through registers. Of 8
+//    waves the two on a SIMD are half a tile apart: one in its products (the scores of a tile, the values of the one before), the
+//    other in its softmax and staging, with a barrier between the halves (8192 rows 592 -> 564 us). Staging is then two
+//    tiles ahead, in four buffers. Workgroups of 4 waves come two a compute unit instead.
 //  * S^T = K . Q^T on v_mfma_scale_f32_32x32x64_f8f6f4: K's codes lie in LDS as they are (a quarter of bf16's LDS reads), their
 //    scale bytes are the product's; q as two e4m3 numbers (see kv4_decode.hip), exact for a bf16 q, at bf16's rate.
 //  * V is widened to bf16 on its way into LDS, transposed as it lies in the cache: a thread takes 8 tokens of two dims, v_cvt applies the
@@ -36,23 +38,33 @@ HS_DEVICE unsigned kv4_no_nan(unsigned w) {  // 255 -> 127
   return w ^ ((((w & 0x7f7f7f7fu) + 0x01010101u) & w & 0x80808080u));
 }
 
-template <int D, int HG, int NWV>
-__global__ __launch_bounds__(64 * NWV) __attribute__((amdgpu_waves_per_eu(2, 8))) void kv4_prefill_kernel(Kv4Attn a, const int* __restrict__ cu_q, int seqs,
-                                                               const int* __restrict__ ctx_lens, int rows,
-                                                               const int* __restrict__ tiles) {
+// A tile in LDS. K's rows are an odd multiple of 16 bytes, V^T's of 16 bytes too: 16 lanes' 16-byte reads on 16 bank groups.
+template <int D>
+struct Kv4Tile {
+  static constexpr int KLD = D == 64 ? 48 : 80, VLD = kKv4Tile + 8;
+  __attribute__((aligned(16))) unsigned short v[D * VLD];
+  __attribute__((aligned(16))) unsigned char k[kKv4Tile * KLD];
+  __attribute__((aligned(16))) unsigned char ks[D / 32][kKv4Tile];  // scale bytes, keys in the cache's order of them
+  __attribute__((aligned(16))) unsigned char vs[D / 32][kKv4Tile];
+  unsigned char nopage[4];                                          // runs of 16 tokens without a page
+};
+
+// kTwo: the two waves of a SIMD are half a tile apart (see above); else every wave is at the same step
+template <int D, int HG, int NWV, bool kTwo>
+__global__ __launch_bounds__(64 * NWV) __attribute__((amdgpu_waves_per_eu(2, 8))) void kv4_prefill_kernel(
+    Kv4Attn a, const int* __restrict__ cu_q, int seqs, const int* __restrict__ ctx_lens, int rows,
+    const int* __restrict__ tiles) {
   constexpr int NG = D / 32, KS = (D + 63) / 64;   // scale groups; steps of the first product
   constexpr int RB = NWV / HG, QR = 32 * RB, SUB = 128 / QR;
   constexpr int NT = 64 * NWV;
-  constexpr int KLD = D == 64 ? 48 : 80;           // bytes of K's LDS rows, an odd multiple of 16: 16 lanes' reads on 16 bank groups
-  constexpr int VLD = kKv4Tile + 8;
-  constexpr int NKI = kKv4Tile * D / 16, NVI = kKv4Tile / 8 * (D / 2);  // 8-byte pieces of K; 8 tokens x 2 dims of V
-  constexpr int NKP = (NKI + NT - 1) / NT, NVP = (NVI + NT - 1) / NT;
-  __shared__ __attribute__((aligned(16))) unsigned char kl[2][kKv4Tile * KLD];
-  __shared__ __attribute__((aligned(16))) unsigned short vl[2][D * VLD];
-  __shared__ unsigned ksc[2][kKv4Tile];                                      // a key's scale bytes, in LDS row order
-  __shared__ __attribute__((aligned(8))) unsigned char vsc[2][NG][kKv4Tile];  // values' scale bytes
-  __shared__ __attribute__((aligned(4))) unsigned char nopage[2][4];                                     // runs of 16 tokens without a page
-  __shared__ int nans;                                                       // a value's scale byte of 255 has come by
+  constexpr int KLD = Kv4Tile<D>::KLD, VLD = Kv4Tile<D>::VLD;
+  constexpr int NKI = kKv4Tile * D / 16, NVI = kKv4Tile / 8 * (D / 2);  // 8-byte pieces of K; 8 tokens x 2 dims of V: as many
+  constexpr int NP = (NKI + NT - 1) / NT;
+  static_assert(NKI == NVI, "one page a thread and piece");
+  constexpr int LEAD = kTwo ? 2 : 1, NBUF = kTwo ? 4 : 2;  // tiles that staging is ahead; buffers
+  extern __shared__ __attribute__((aligned(16))) char smem[];
+  Kv4Tile<D>* buf = reinterpret_cast<Kv4Tile<D>*>(smem);
+  __shared__ int nans;  // a value's scale byte of 255 has come by
 
   // dispatch order: kv-head groups fastest, then the host's tiles, the later rows of a tile first
   const int L = blockIdx.x + gridDim.x * blockIdx.y, gy = gridDim.y;
@@ -69,7 +81,6 @@ __global__ __launch_bounds__(64 * NWV) __attribute__((amdgpu_waves_per_eu(2, 8))
   const int h = gyi * HG + wave % HG;
   const int qi = lane & 31, half = lane >> 5;
   const int wrow0 = r0 + wave / HG * 32;
-  const bool wactive = wrow0 < qlen;
   const int row = min(wrow0 + qi, qlen - 1);
   const int pos = ctx - qlen + row;                                    // this lane's row
   const int wmin = ctx - qlen + wrow0, wmax = ctx - qlen + min(wrow0 + 31, qlen - 1);  // the wave's
@@ -83,98 +94,80 @@ __global__ __launch_bounds__(64 * NWV) __attribute__((amdgpu_waves_per_eu(2, 8))
   const int* bt = a.block_tables + (long)seq * a.bt_stride;
   const int bsh = __builtin_ctz(bs), bmask = bs - 1;
 
-  // ---- staging. Pages are asked for a tile before the loads that need them.
+  // ---- staging: a thread's pieces of K and V are of one run of 16 tokens (K: a key's 16 dims; V: 8 tokens of two dims), so of one
+  // page, asked for a tile before the loads that need it. Threads past the pieces load others' again and store nothing.
   const long head_bytes = kv4_head_bytes(bs, D), page_bytes = head_bytes * nkv;
   const int code_bytes = kv4_code_bytes(bs, D);
   const unsigned char* kbase = static_cast<const unsigned char*>(a.cache.k) + kh * head_bytes;
   const unsigned char* vbase = static_cast<const unsigned char*>(a.cache.v) + kh * head_bytes;
-  struct Pages {
-    int k[NKP], v[NVP], s;
-  };
+  int pg[NP];
   struct Stage {
-    u32x2 k[NKP], v[NVP], vs[NVP];
-    unsigned ks;
-    int vpage[NVP];
+    u32x2 k[NP], v[NP], vs[NP];
+    u32x4 ks[NP];  // threads in < NG: the scale bytes of a run's keys
+    bool page[NP];
   };
-  auto pages = [&](int v, Pages& pg) {
+  auto run_of = [&](int i) { return (tid + NT * i) / D; };
+  auto in_of = [&](int i) { return (tid + NT * i) % D; };
+  auto pages = [&](int v) {
     const int key = tile_key(min(v, nkt - 1));
 #pragma unroll
-    for (int i = 0; i < NKP; ++i) pg.k[i] = bt[min(key + (tid + NT * i) / (D / 16) % kKv4Tile, last) >> bsh];
-#pragma unroll
-    for (int i = 0; i < NVP; ++i) pg.v[i] = bt[min(key + 16 * ((tid + NT * i) / D % 4), last) >> bsh];
-    pg.s = bt[min(key + lane, last) >> bsh];
+    for (int i = 0; i < NP; ++i) pg[i] = bt[min(key + 16 * (run_of(i) & 3), last) >> bsh];
   };
-  auto load = [&](int v, const Pages& pg, Stage& st) {
+  auto load = [&](int v, Stage& s) {
     const int key = tile_key(min(v, nkt - 1));
 #pragma unroll
-    for (int i = 0; i < NKP; ++i) {
-      const int it = tid + NT * i, kk = it / (D / 16) % kKv4Tile, piece = it % (D / 16);
-      st.k[i] = *reinterpret_cast<const u32x2*>(kbase + (long)max(kv4_page(pg.k[i], a.cache.blocks), 0) * page_bytes +
-                                                ((key + kk) & bmask) * (D / 2) + 8 * piece);
-    }
-#pragma unroll
-    for (int i = 0; i < NVP; ++i) {
-      const int it = tid + NT * i, run = it / D % 4, p = it % D >> 1, h8 = it & 1;
-      const int page = kv4_page(pg.v[i], a.cache.blocks), off = ((key + 16 * run) & bmask) + 8 * h8;
-      const unsigned char* vp = vbase + (long)max(page, 0) * page_bytes;
-      st.v[i] = *reinterpret_cast<const u32x2*>(vp + p * bs + off);
-      st.vs[i] = *reinterpret_cast<const u32x2*>(vp + code_bytes + (p >> 4) * bs + off);
-      st.vpage[i] = page;
-    }
-    if (wave == 0) {  // a key's scale bytes, together
-      const unsigned char* sp = kbase + (long)max(kv4_page(pg.s, a.cache.blocks), 0) * page_bytes + code_bytes +
-                                kv4_key_scale_at((key + lane) & bmask);
-      unsigned w = 0;
-#pragma unroll
-      for (int g = 0; g < 4; ++g) w |= (g < NG ? (unsigned)sp[g * bs] : 127u) << (8 * g);
-      st.ks = w;
+    for (int i = 0; i < NP; ++i) {
+      const int page = kv4_page(pg[i], a.cache.blocks), off = (key + 16 * (run_of(i) & 3)) & bmask, in = in_of(i);
+      const long at = (long)max(page, 0) * page_bytes;
+      const unsigned char *kp = kbase + at, *vp = vbase + at + off;
+      s.page[i] = page >= 0;
+      s.k[i] = *reinterpret_cast<const u32x2*>(kp + (off + in / (D / 16)) * (D / 2) + 8 * (in % (D / 16)));
+      s.v[i] = *reinterpret_cast<const u32x2*>(vp + (in >> 1) * bs + 8 * (in & 1));
+      s.vs[i] = *reinterpret_cast<const u32x2*>(vp + code_bytes + (in >> 5) * bs + 8 * (in & 1));
+      if (in < NG) s.ks[i] = *reinterpret_cast<const u32x4*>(kp + code_bytes + in * bs + off);
     }
   };
-  auto store = [&](Stage& st, int buf) {
+  auto store = [&](Stage& s, Kv4Tile<D>& b) {
 #pragma unroll
-    for (int i = 0; i < NKP; ++i) {
-      const int it = tid + NT * i, kk = it / (D / 16), piece = it % (D / 16);
-      const int krow = (kk & ~12) | ((kk & 4) << 1) | ((kk & 8) >> 1);
-      if (NKI % NT == 0 || it < NKI) *reinterpret_cast<u32x2*>(&kl[buf][krow * KLD + 8 * piece]) = st.k[i];
-    }
-    if (wave == 0) ksc[buf][(lane & ~12) | ((lane & 4) << 1) | ((lane & 8) >> 1)] = st.ks;
-#pragma unroll
-    for (int i = 0; i < NVP; ++i) {
-      const int it = tid + NT * i, run = it / D, p = it % D >> 1, h8 = it & 1;
-      if (NVI % NT != 0 && it >= NVI) continue;
-      if ((p & 15) == 0) *reinterpret_cast<u32x2*>(&vsc[buf][p >> 4][16 * run + 8 * h8]) = st.vs[i];
-      if ((it % D) == 0) nopage[buf][run] = st.vpage[i] < 0;
-      if (kv4_any_nan(st.vs[i][0]) || kv4_any_nan(st.vs[i][1])) {
+    for (int i = 0; i < NP; ++i) {
+      const int run = run_of(i), in = in_of(i);
+      if (NKI % NT != 0 && run > 3) continue;
+      const int kk = 16 * run + in / (D / 16), krow = (kk & ~12) | ((kk & 4) << 1) | ((kk & 8) >> 1);
+      *reinterpret_cast<u32x2*>(&b.k[krow * KLD + 8 * (in % (D / 16))]) = s.k[i];
+      if (in < NG) *reinterpret_cast<u32x4*>(&b.ks[in][16 * run]) = s.ks[i];
+      if (in == 0) b.nopage[run] = !s.page[i];
+      if ((in & 30) == 0) *reinterpret_cast<u32x2*>(&b.vs[in >> 5][16 * run + 8 * (in & 1)]) = s.vs[i];
+      if (kv4_any_nan(s.vs[i][0]) || kv4_any_nan(s.vs[i][1])) {
         nans = 1;
-        st.vs[i][0] = kv4_no_nan(st.vs[i][0]);
-        st.vs[i][1] = kv4_no_nan(st.vs[i][1]);
+        s.vs[i][0] = kv4_no_nan(s.vs[i][0]);
+        s.vs[i][1] = kv4_no_nan(s.vs[i][1]);
       }
       u32x4 even, odd;
 #pragma unroll
       for (int q = 0; q < 2; ++q) {
-        const unsigned w = st.v[i][q], s = st.vs[i][q];
-        const unsigned x0 = kv4_widen2<0>(w, __uint_as_float(s << 23)), x1 = kv4_widen2<1>(w, __uint_as_float(s << 15));
-        const unsigned x2 = kv4_widen2<2>(w, __uint_as_float(s << 7)), x3 = kv4_widen2<3>(w, __uint_as_float(s >> 1));
+        const unsigned w = s.v[i][q], c = s.vs[i][q];
+        const unsigned x0 = kv4_widen2<0>(w, __uint_as_float(c << 23)), x1 = kv4_widen2<1>(w, __uint_as_float(c << 15));
+        const unsigned x2 = kv4_widen2<2>(w, __uint_as_float(c << 7)), x3 = kv4_widen2<3>(w, __uint_as_float(c >> 1));
         even[2 * q] = __builtin_amdgcn_perm(x1, x0, 0x05040100u);
         odd[2 * q] = __builtin_amdgcn_perm(x1, x0, 0x07060302u);
         even[2 * q + 1] = __builtin_amdgcn_perm(x3, x2, 0x05040100u);
         odd[2 * q + 1] = __builtin_amdgcn_perm(x3, x2, 0x07060302u);
       }
-      unsigned short* dst = &vl[buf][2 * p * VLD + 16 * run + 8 * h8];
+      unsigned short* dst = &b.v[(in & ~1) * VLD + 16 * run + 8 * (in & 1)];
       *reinterpret_cast<u32x4*>(dst) = even;
       *reinterpret_cast<u32x4*>(dst + VLD) = odd;
     }
   };
 
-  Pages pg;
-  Stage sa, sb;
+  Stage stage, stage1;
   if (nkt > 0) {
-    pages(0, pg);
-    Pages next;
-    pages(1, next);
-    load(0, pg, sa);
-    pages(2, pg);
-    load(1, next, sb);
+    pages(0);
+    load(0, stage);
+    if (kTwo) {
+      pages(1);
+      load(1, stage1);
+    }
+    pages(LEAD);
   }
 
   // ---- q of this lane's row: dims 64 s + 16 half .. and 64 s + 32 + 16 half .. of step s
@@ -210,45 +203,50 @@ __global__ __launch_bounds__(64 * NWV) __attribute__((amdgpu_waves_per_eu(2, 8))
       }
   }
 
-  f32x16 o[NG];
+  f32x16 o[NG], st[2];
+  bf16x8 pb[4];  // P of 16 keys a step
 #pragma unroll
   for (int nb = 0; nb < NG; ++nb)
 #pragma unroll
     for (int r = 0; r < 16; ++r) o[nb][r] = 0.f;
   float m_run = -1e30f, l_run = 0.f;
 
-  auto compute = [&](int v, int buf) __attribute__((always_inline)) {
+  auto sees_some = [&](int v) {  // whether a row of the wave may see a key of tile v
     const int key = tile_key(v);
-    if (!wactive || key > wmax || (window > 0 && key + kKv4Tile - 1 <= wmin - window && key >= sinks)) return;
-    const unsigned gone = __builtin_amdgcn_readfirstlane(*reinterpret_cast<const unsigned*>(nopage[buf]));
-    const int bad = __builtin_amdgcn_readfirstlane(nans);
-    // ---- scores: rows (keys) of the tile's halves, columns (queries) qi
-    f32x16 st[2];
+    return wrow0 < qlen && key <= wmax && (window <= 0 || key + kKv4Tile - 1 > wmin - window || key < sinks);
+  };
+  // scores: rows (keys) of the tile's halves, columns (queries) qi. Key 16 j + o of a half lies in row 16 j + r with o's bits 2 and 3
+  // exchanged, and its scale byte at 16 j + 4 (o % 4) + o / 4
+  const int ks_at = (qi & 16) | ((qi & 3) << 2) | ((qi >> 1) & 2) | ((qi >> 3) & 1);
+  auto scores = [&](const Kv4Tile<D>& b) __attribute__((always_inline)) {
 #pragma unroll
     for (int h2 = 0; h2 < 2; ++h2)
 #pragma unroll
       for (int r = 0; r < 16; ++r) st[h2][r] = 0.f;
-    unsigned ks[2];
-#pragma unroll
-    for (int h2 = 0; h2 < 2; ++h2) ks[h2] = ksc[buf][32 * h2 + qi] >> (8 * half);
 #pragma unroll
     for (int s = 0; s < KS; ++s) {
+      const int g = min(2 * s + half, NG - 1);
       u32x4 kf[2];
+      int ks[2];
 #pragma unroll
-      for (int h2 = 0; h2 < 2; ++h2)
-        kf[h2] = *reinterpret_cast<const u32x4*>(&kl[buf][(32 * h2 + qi) * KLD + 16 * min(2 * s + half, NG - 1)]);
+      for (int h2 = 0; h2 < 2; ++h2) {
+        kf[h2] = *reinterpret_cast<const u32x4*>(&b.k[(32 * h2 + qi) * KLD + 16 * g]);
+        ks[h2] = b.ks[g][32 * h2 + ks_at];
+        if (D == 96 && s == 1 && half) ks[h2] = 127;  // no such dims: q is zero there, whatever the scale of others is
+      }
 #pragma unroll
       for (int part = 0; part < 2; ++part)
 #pragma unroll
-        for (int h2 = 0; h2 < 2; ++h2) {
-          const i32x8 ka{(int)kf[h2][0], (int)kf[h2][1], (int)kf[h2][2], (int)kf[h2][3], 0, 0, 0, 0};
-          const i32x8 qb = part == 0 ? qlo[s] : qhi[s];
-          const int qs = part == 0 ? 123 : 127;
-          if (s == 0) st[h2] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(ka, qb, st[h2], 4, 0, 0, (int)ks[h2], 0, qs);
-          else st[h2] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(ka, qb, st[h2], 4, 0, 2, (int)ks[h2], 0, qs);
-        }
+        for (int h2 = 0; h2 < 2; ++h2)
+          st[h2] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(
+              i32x8{(int)kf[h2][0], (int)kf[h2][1], (int)kf[h2][2], (int)kf[h2][3], 0, 0, 0, 0},
+              part == 0 ? qlo[s] : qhi[s], st[h2], 4, 0, 0, ks[h2], 0, part == 0 ? 123 : 127);
     }
-    // ---- hidden keys, in tiles that some row of the wave does not see whole; slot (h2, r): key 32 h2 + 16 (r >> 3) + 8 half + (r & 7)
+  };
+  auto softmax = [&](int v, const Kv4Tile<D>& b) __attribute__((always_inline)) {
+    const int key = tile_key(v);
+    const unsigned gone = __builtin_amdgcn_readfirstlane(*reinterpret_cast<const unsigned*>(b.nopage));
+    // hidden keys, in tiles that some row of the wave does not see whole; slot (h2, r): key 32 h2 + 16 (r >> 3) + 8 half + (r & 7)
     const bool whole = key + kKv4Tile - 1 <= min(wmin, cap - 1) &&
                        (window <= 0 || key > wmax - window || key + kKv4Tile <= sinks) && gone == 0;
     if (!whole) {
@@ -293,34 +291,38 @@ __global__ __launch_bounds__(64 * NWV) __attribute__((amdgpu_waves_per_eu(2, 8))
 #pragma unroll
         for (int r = 0; r < 16; ++r) o[nb][r] *= alpha;
     }
+    // the sum is that of the rounded P, two at a time
     float ps[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-    for (int h2 = 0; h2 < 2; ++h2) {
-      bf16x8 pb[2];
-#pragma unroll
-      for (int r = 0; r < 16; ++r) {
-        const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(st[h2][r], sl, -m_run));
-        ps[r & 3] += p;
-        pb[r >> 3][r & 7] = static_cast<__bf16>(p);
-      }
-#pragma unroll
-      for (int s2 = 0; s2 < 2; ++s2) {
-        const unsigned short* vb = &vl[buf][qi * VLD + 32 * h2 + 16 * s2 + 8 * half];
-#pragma unroll
-        for (int nb = 0; nb < NG; ++nb) {
-          const u16x8 va = *reinterpret_cast<const u16x8*>(vb + 32 * nb * VLD);
-          o[nb] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, va), pb[s2], o[nb], 0, 0, 0);
-        }
-      }
+    for (int i = 0; i < 32; i += 2) {
+      const f32x16& x = st[i >> 4];
+      const bf16x2 p{static_cast<__bf16>(__builtin_amdgcn_exp2f(__builtin_fmaf(x[i & 15], sl, -m_run))),
+                     static_cast<__bf16>(__builtin_amdgcn_exp2f(__builtin_fmaf(x[(i & 15) + 1], sl, -m_run)))};
+      ps[(i >> 1) & 3] = __builtin_amdgcn_fdot2_f32_bf16(p, bf16x2{static_cast<__bf16>(1.f), static_cast<__bf16>(1.f)}, ps[(i >> 1) & 3], false);
+      pb[i >> 3][i & 7] = p[0];
+      pb[i >> 3][(i & 7) + 1] = p[1];
     }
     l_run += (ps[0] + ps[1]) + (ps[2] + ps[3]);
-    if (bad) {  // values of NaN among this tile's: into the rows that see them
-      unsigned long seen = 0;
-      for (int j = 0; j < kKv4Tile; ++j)
-        if (key + j < cap && !(gone >> (8 * (j >> 4)) & 255u) && kv4_sees(key + j, pos, window, sinks)) seen |= 1ul << j;
+  };
+  auto values = [&](int v, const Kv4Tile<D>& b) __attribute__((always_inline)) {
+    const int bad = __builtin_amdgcn_readfirstlane(nans);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const unsigned short* vb = &b.v[qi * VLD + 16 * j + 8 * half];
 #pragma unroll
       for (int nb = 0; nb < NG; ++nb) {
-        const unsigned long lost = __ballot(vsc[buf][nb][lane] == kKv4Nan);
+        const u16x8 va = *reinterpret_cast<const u16x8*>(vb + 32 * nb * VLD);
+        o[nb] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, va), pb[j], o[nb], 0, 0, 0);
+      }
+    }
+    if (bad) {  // values of NaN may be among this tile's: into the rows that see them
+      const int key = tile_key(v);
+      unsigned long seen = 0;
+      for (int j = 0; j < kKv4Tile; ++j)
+        if (key + j < cap && !b.nopage[j >> 4] && kv4_sees(key + j, pos, window, sinks)) seen |= 1ul << j;
+#pragma unroll
+      for (int nb = 0; nb < NG; ++nb) {
+        const unsigned long lost = __ballot(b.vs[nb][lane] == kKv4Nan);
         if (seen & lost)
 #pragma unroll
           for (int r = 0; r < 16; ++r) o[nb][r] = NAN;
@@ -330,24 +332,30 @@ __global__ __launch_bounds__(64 * NWV) __attribute__((amdgpu_waves_per_eu(2, 8))
 
   if (tid == 0) nans = 0;
   __syncthreads();
-  if (nkt > 0) store(sa, 0);
+  if (nkt > 0) {
+    store(stage, buf[0]);
+    if (kTwo) store(stage1, buf[1]);
+    load(LEAD, stage);
+    pages(LEAD + 1);
+  }
   __syncthreads();
-  for (int v = 0; v < nkt; v += 2) {
-    // tile v in buffer 0; sb holds tile v + 1; pg the pages of tile v + 2
-    Pages next;
-    pages(v + 3, next);
-    load(v + 2, pg, sa);
-    compute(v, 0);
-    if (v + 1 < nkt) store(sb, 1);
+  const bool later = kTwo && wave >= NWV / 2;
+  if (later) __syncthreads();
+  bool live = false;  // whether the tile before has P
+  for (int v = 0; v < nkt; ++v) {
+    if (live) values(v - 1, buf[(v - 1) & (NBUF - 1)]);
+    live = sees_some(v);
+    if (live) scores(buf[v & (NBUF - 1)]);
     __syncthreads();
-    if (v + 1 >= nkt) break;
-    pages(v + 4, pg);
-    load(v + 3, next, sb);
-    compute(v + 1, 1);
-    if (v + 2 < nkt) store(sa, 0);
+    if (live) softmax(v, buf[v & (NBUF - 1)]);
+    store(stage, buf[(v + LEAD) & (NBUF - 1)]);
+    load(v + LEAD + 1, stage);
+    pages(v + LEAD + 2);
     __syncthreads();
   }
-  if (!wactive || wrow0 + qi >= qlen) return;
+  if (live) values(nkt - 1, buf[(nkt - 1) & (NBUF - 1)]);
+  if (kTwo && !later) __syncthreads();
+  if (wrow0 + qi >= qlen) return;
   l_run = kv4_sum32(l_run);
   const float inv = l_run == 0.f ? 0.f : 1.f / l_run;  // a row that sees nothing: zeros
   unsigned short* op = static_cast<unsigned short*>(a.out) + (long)(q0 + row) * a.out_stride + (long)h * D;
@@ -366,7 +374,12 @@ template <int D, int HG, int NWV>
 static void kv4_prefill(const Kv4Attn& a, const int* cu_q, int seqs, const int* ctx, int rows, const int* tiles, int ntiles,
                         hipStream_t s) {
   constexpr int SUB = 128 / (32 * (NWV / HG));
-  kv4_prefill_kernel<D, HG, NWV><<<dim3(ntiles * SUB, a.nq / HG), 64 * NWV, 0, s>>>(a, cu_q, seqs, ctx, rows, tiles);
+  constexpr bool kTwo = NWV == 8;
+  constexpr int kLds = (kTwo ? 4 : 2) * sizeof(Kv4Tile<D>);
+  static const bool attr [[maybe_unused]] =
+      hipFuncSetAttribute(reinterpret_cast<const void*>(&kv4_prefill_kernel<D, HG, NWV, kTwo>),
+                          hipFuncAttributeMaxDynamicSharedMemorySize, kLds) == hipSuccess;
+  kv4_prefill_kernel<D, HG, NWV, kTwo><<<dim3(ntiles * SUB, a.nq / HG), 64 * NWV, kLds, s>>>(a, cu_q, seqs, ctx, rows, tiles);
 }
 
 // as many query heads a workgroup as divide a kv head's, up to 8 waves
