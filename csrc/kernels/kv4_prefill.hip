@@ -50,7 +50,7 @@ struct Kv4Tile {
 };
 
 // kTwo: the two waves of a SIMD are half a tile apart (see above); else every wave is at the same step
-template <int D, int HG, int NWV, bool kTwo>
+template <int D, int HG, int NWV, int UN>
 __global__ __launch_bounds__(64 * NWV) __attribute__((amdgpu_waves_per_eu(2, 8))) void kv4_prefill_kernel(
     Kv4Attn a, const int* __restrict__ cu_q, int seqs, const int* __restrict__ ctx_lens, int rows,
     const int* __restrict__ tiles) {
@@ -58,10 +58,7 @@ __global__ __launch_bounds__(64 * NWV) __attribute__((amdgpu_waves_per_eu(2, 8))
   constexpr int RB = NWV / HG, QR = 32 * RB, SUB = 128 / QR;
   constexpr int NT = 64 * NWV;
   constexpr int KLD = Kv4Tile<D>::KLD, VLD = Kv4Tile<D>::VLD;
-  constexpr int NKI = kKv4Tile * D / 16, NVI = kKv4Tile / 8 * (D / 2);  // 8-byte pieces of K; 8 tokens x 2 dims of V: as many
-  constexpr int NP = (NKI + NT - 1) / NT;
-  static_assert(NKI == NVI, "one page a thread and piece");
-  constexpr int LEAD = kTwo ? 2 : 1, NBUF = kTwo ? 4 : 2;  // tiles that staging is ahead; buffers
+  constexpr int NP = 512 / NT;  // runs of a tile that two waves take
   extern __shared__ __attribute__((aligned(16))) char smem[];
   Kv4Tile<D>* buf = reinterpret_cast<Kv4Tile<D>*>(smem);
   __shared__ int nans;  // a value's scale byte of 255 has come by
@@ -94,58 +91,54 @@ __global__ __launch_bounds__(64 * NWV) __attribute__((amdgpu_waves_per_eu(2, 8))
   const int* bt = a.block_tables + (long)seq * a.bt_stride;
   const int bsh = __builtin_ctz(bs), bmask = bs - 1;
 
-  // ---- staging: a thread's pieces of K and V are of one run of 16 tokens (K: a key's 16 dims; V: 8 tokens of two dims), so of one
-  // page, asked for a tile before the loads that need it. Threads past the pieces load others' again and store nothing.
+  // ---- staging: two waves take a run of 16 tokens, a lane of the first D a key's 16 dims and 8 tokens of two dims. The run's page is
+  // the same for a wave, so that addresses are scalars; it is asked for a step before the loads that need it.
   const long head_bytes = kv4_head_bytes(bs, D), page_bytes = head_bytes * nkv;
   const int code_bytes = kv4_code_bytes(bs, D);
   const unsigned char* kbase = static_cast<const unsigned char*>(a.cache.k) + kh * head_bytes;
   const unsigned char* vbase = static_cast<const unsigned char*>(a.cache.v) + kh * head_bytes;
-  int pg[NP];
   struct Stage {
     u32x2 k[NP], v[NP], vs[NP];
-    u32x4 ks[NP];  // threads in < NG: the scale bytes of a run's keys
+    u32x4 ks[NP];  // lanes in < NG: the scale bytes of a run's keys
     bool page[NP];
   };
-  auto run_of = [&](int i) { return (tid + NT * i) / D; };
-  auto in_of = [&](int i) { return (tid + NT * i) % D; };
-  auto pages = [&](int v) {
+  const int in = tid & 127;
+  const int kin = (in / (D / 16)) * (D / 2) + 8 * (in % (D / 16)), vin = (in >> 1) * bs + 8 * (in & 1);
+  const int sin = (in >> 5) * bs + 8 * (in & 1), ksin = in * bs;
+  auto run_of = [&](int i) { return (wave >> 1) + NT / 128 * i; };
+  auto pages = [&](int v, int (&pg)[NP]) {
     const int key = tile_key(min(v, nkt - 1));
 #pragma unroll
-    for (int i = 0; i < NP; ++i) pg[i] = bt[min(key + 16 * (run_of(i) & 3), last) >> bsh];
+    for (int i = 0; i < NP; ++i) pg[i] = bt[min(key + 16 * run_of(i), last) >> bsh];
   };
-  auto load = [&](int v, Stage& s) {
+  auto load = [&](int v, const int (&pg)[NP], Stage& s) {
     const int key = tile_key(min(v, nkt - 1));
 #pragma unroll
     for (int i = 0; i < NP; ++i) {
-      const int page = kv4_page(pg[i], a.cache.blocks), off = (key + 16 * (run_of(i) & 3)) & bmask, in = in_of(i);
+      const int page = kv4_page(pg[i], a.cache.blocks), off = (key + 16 * run_of(i)) & bmask;
       const long at = (long)max(page, 0) * page_bytes;
       const unsigned char *kp = kbase + at, *vp = vbase + at + off;
       s.page[i] = page >= 0;
-      s.k[i] = *reinterpret_cast<const u32x2*>(kp + (off + in / (D / 16)) * (D / 2) + 8 * (in % (D / 16)));
-      s.v[i] = *reinterpret_cast<const u32x2*>(vp + (in >> 1) * bs + 8 * (in & 1));
-      s.vs[i] = *reinterpret_cast<const u32x2*>(vp + code_bytes + (in >> 5) * bs + 8 * (in & 1));
-      if (in < NG) s.ks[i] = *reinterpret_cast<const u32x4*>(kp + code_bytes + in * bs + off);
+      if (D == 128 || in < D) {
+        s.k[i] = *reinterpret_cast<const u32x2*>(kp + off * (D / 2) + (unsigned)kin);
+        s.v[i] = *reinterpret_cast<const u32x2*>(vp + (unsigned)vin);
+        s.vs[i] = *reinterpret_cast<const u32x2*>(vp + code_bytes + (unsigned)sin);
+      }
+      if (in < NG) s.ks[i] = *reinterpret_cast<const u32x4*>(kp + code_bytes + off + (unsigned)ksin);
     }
   };
-  auto store = [&](Stage& s, Kv4Tile<D>& b) {
+  // what every thread does, without a branch, and the few that have more
+  auto store = [&](Stage& s, Kv4Tile<D>& b) __attribute__((always_inline)) {
 #pragma unroll
     for (int i = 0; i < NP; ++i) {
-      const int run = run_of(i), in = in_of(i);
-      if (NKI % NT != 0 && run > 3) continue;
+      const int run = run_of(i);
+      if (D != 128 && in >= D) continue;
       const int kk = 16 * run + in / (D / 16), krow = (kk & ~12) | ((kk & 4) << 1) | ((kk & 8) >> 1);
       *reinterpret_cast<u32x2*>(&b.k[krow * KLD + 8 * (in % (D / 16))]) = s.k[i];
-      if (in < NG) *reinterpret_cast<u32x4*>(&b.ks[in][16 * run]) = s.ks[i];
-      if (in == 0) b.nopage[run] = !s.page[i];
-      if ((in & 30) == 0) *reinterpret_cast<u32x2*>(&b.vs[in >> 5][16 * run + 8 * (in & 1)]) = s.vs[i];
-      if (kv4_any_nan(s.vs[i][0]) || kv4_any_nan(s.vs[i][1])) {
-        nans = 1;
-        s.vs[i][0] = kv4_no_nan(s.vs[i][0]);
-        s.vs[i][1] = kv4_no_nan(s.vs[i][1]);
-      }
       u32x4 even, odd;
 #pragma unroll
       for (int q = 0; q < 2; ++q) {
-        const unsigned w = s.v[i][q], c = s.vs[i][q];
+        const unsigned w = s.v[i][q], c = kv4_no_nan(s.vs[i][q]);
         const unsigned x0 = kv4_widen2<0>(w, __uint_as_float(c << 23)), x1 = kv4_widen2<1>(w, __uint_as_float(c << 15));
         const unsigned x2 = kv4_widen2<2>(w, __uint_as_float(c << 7)), x3 = kv4_widen2<3>(w, __uint_as_float(c >> 1));
         even[2 * q] = __builtin_amdgcn_perm(x1, x0, 0x05040100u);
@@ -158,16 +151,34 @@ __global__ __launch_bounds__(64 * NWV) __attribute__((amdgpu_waves_per_eu(2, 8))
       *reinterpret_cast<u32x4*>(dst + VLD) = odd;
     }
   };
-
-  Stage stage, stage1;
-  if (nkt > 0) {
-    pages(0);
-    load(0, stage);
-    if (kTwo) {
-      pages(1);
-      load(1, stage1);
+  auto store_scales = [&](const Stage& s, Kv4Tile<D>& b) __attribute__((always_inline)) {
+#pragma unroll
+    for (int i = 0; i < NP; ++i) {
+      const int run = run_of(i);
+      if (D != 128 && in >= D) continue;
+      if ((in & 30) == 0) {
+        *reinterpret_cast<u32x2*>(&b.vs[in >> 5][16 * run + 8 * (in & 1)]) = s.vs[i];
+        if (kv4_any_nan(s.vs[i][0]) || kv4_any_nan(s.vs[i][1])) nans = 1;
+      }
+      if (in < NG) *reinterpret_cast<u32x4*>(&b.ks[in][16 * run]) = s.ks[i];
+      if (in == 0) b.nopage[run] = !s.page[i];
     }
-    pages(LEAD);
+  };
+
+  Stage stage[UN];
+  int pgs[UN][NP];
+  auto ask = [&](int v) {  // the pages of tiles v .. v + UN - 1
+#pragma unroll
+    for (int u = 0; u < UN; ++u) pages(v + u, pgs[u]);
+  };
+  auto fetch = [&](int v) {
+#pragma unroll
+    for (int u = 0; u < UN; ++u) load(v + u, pgs[u], stage[u]);
+  };
+  if (nkt > 0) {
+    ask(0);
+    fetch(0);
+    ask(UN);
   }
 
   // ---- q of this lane's row: dims 64 s + 16 half .. and 64 s + 32 + 16 half .. of step s
@@ -332,29 +343,73 @@ __global__ __launch_bounds__(64 * NWV) __attribute__((amdgpu_waves_per_eu(2, 8))
 
   if (tid == 0) nans = 0;
   __syncthreads();
-  if (nkt > 0) {
-    store(stage, buf[0]);
-    if (kTwo) store(stage1, buf[1]);
-    load(LEAD, stage);
-    pages(LEAD + 1);
-  }
-  __syncthreads();
-  const bool later = kTwo && wave >= NWV / 2;
-  if (later) __syncthreads();
-  bool live = false;  // whether the tile before has P
-  for (int v = 0; v < nkt; ++v) {
-    if (live) values(v - 1, buf[(v - 1) & (NBUF - 1)]);
-    live = sees_some(v);
-    if (live) scores(buf[v & (NBUF - 1)]);
+  if constexpr (NWV == 8) {
+    // two tiles a barrier. Half of the waves stage the next ones before their products, the others after them, so that the two waves of a
+    // SIMD are at different work
+    auto put = [&](int at) {
+#pragma unroll
+      for (int u = 0; u < UN; ++u) {
+        store(stage[u], buf[at + u]);
+        store_scales(stage[u], buf[at + u]);
+      }
+    };
+    auto tile = [&](int v, const Kv4Tile<D>& b) __attribute__((always_inline)) {
+      if (!sees_some(v)) return;
+      scores(b);
+      softmax(v, b);
+      values(v, b);
+    };
+    if (nkt > 0) {
+      put(0);
+      fetch(UN);
+      ask(2 * UN);
+    }
     __syncthreads();
-    if (live) softmax(v, buf[v & (NBUF - 1)]);
-    store(stage, buf[(v + LEAD) & (NBUF - 1)]);
-    load(v + LEAD + 1, stage);
-    pages(v + LEAD + 2);
+    const bool early = wave >= NWV / 2;
+    int at = 0;
+    for (int v = 0; v < nkt; v += UN) {
+      const int next = UN - at;
+      if (early) {
+        put(next);
+        fetch(v + 2 * UN);
+        ask(v + 3 * UN);
+      }
+#pragma unroll 1
+      for (int u = 0; u < UN; ++u)
+        if (u == 0 || v + u < nkt) tile(v + u, buf[at + u]);
+      if (!early) {
+        put(next);
+        fetch(v + 2 * UN);
+        ask(v + 3 * UN);
+      }
+      at = next;
+      __syncthreads();
+    }
+  } else {
+    // the values of a tile and the scores of the next one together; workgroups come two a compute unit
+    if (nkt > 0) {
+      store(stage[0], buf[0]);
+      store_scales(stage[0], buf[0]);
+      fetch(1);
+      ask(2);
+    }
     __syncthreads();
+    bool live = false;  // whether the tile before has P
+    for (int v = 0; v < nkt; ++v) {
+      Kv4Tile<D>&b0 = buf[v & 1], &b1 = buf[~v & 1];
+      if (live) values(v - 1, b1);
+      live = sees_some(v);
+      if (live) scores(b0);
+      __syncthreads();
+      if (live) softmax(v, b0);
+      store(stage[0], b1);
+      store_scales(stage[0], b1);
+      fetch(v + 2);
+      ask(v + 3);
+      __syncthreads();
+    }
+    if (live) values(nkt - 1, buf[(nkt - 1) & 1]);
   }
-  if (live) values(nkt - 1, buf[(nkt - 1) & (NBUF - 1)]);
-  if (kTwo && !later) __syncthreads();
   if (wrow0 + qi >= qlen) return;
   l_run = kv4_sum32(l_run);
   const float inv = l_run == 0.f ? 0.f : 1.f / l_run;  // a row that sees nothing: zeros
@@ -374,12 +429,12 @@ template <int D, int HG, int NWV>
 static void kv4_prefill(const Kv4Attn& a, const int* cu_q, int seqs, const int* ctx, int rows, const int* tiles, int ntiles,
                         hipStream_t s) {
   constexpr int SUB = 128 / (32 * (NWV / HG));
-  constexpr bool kTwo = NWV == 8;
-  constexpr int kLds = (kTwo ? 4 : 2) * sizeof(Kv4Tile<D>);
+  constexpr int UN = NWV == 8 ? 2 : 1;  // workgroups of 4 waves come two a compute unit
+  constexpr int kLds = 2 * UN * sizeof(Kv4Tile<D>);
   static const bool attr [[maybe_unused]] =
-      hipFuncSetAttribute(reinterpret_cast<const void*>(&kv4_prefill_kernel<D, HG, NWV, kTwo>),
+      hipFuncSetAttribute(reinterpret_cast<const void*>(&kv4_prefill_kernel<D, HG, NWV, UN>),
                           hipFuncAttributeMaxDynamicSharedMemorySize, kLds) == hipSuccess;
-  kv4_prefill_kernel<D, HG, NWV, kTwo><<<dim3(ntiles * SUB, a.nq / HG), 64 * NWV, kLds, s>>>(a, cu_q, seqs, ctx, rows, tiles);
+  kv4_prefill_kernel<D, HG, NWV, UN><<<dim3(ntiles * SUB, a.nq / HG), 64 * NWV, kLds, s>>>(a, cu_q, seqs, ctx, rows, tiles);
 }
 
 // as many query heads a workgroup as divide a kv head's, up to 8 waves
