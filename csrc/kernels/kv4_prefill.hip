@@ -91,6 +91,19 @@ __global__ __launch_bounds__(64 * NWV) __attribute__((amdgpu_waves_per_eu(2, 8))
   const int* bt = a.block_tables + (long)seq * a.bt_stride;
   const int bsh = __builtin_ctz(bs), bmask = bs - 1;
 
+  // ---- q of this lane's row, on its way first: dims 64 s + 16 half .. and 64 s + 32 + 16 half .. of step s
+  u16x8 raw[KS][4];
+  {
+    const unsigned short* qp = static_cast<const unsigned short*>(a.q) + (long)(q0 + row) * a.q_stride + (long)h * D + 16 * half;
+#pragma unroll
+    for (int s = 0; s < KS; ++s)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const int d0 = 64 * s + 32 * (e >> 1) + 8 * (e & 1);
+        raw[s][e] = d0 < D ? *reinterpret_cast<const u16x8*>(qp + d0) : u16x8{0, 0, 0, 0, 0, 0, 0, 0};
+      }
+  }
+
   // ---- staging: two waves take a run of 16 tokens, a lane of the first D a key's 16 dims and 8 tokens of two dims. The run's page is
   // the same for a wave, so that addresses are scalars; it is asked for a step before the loads that need it.
   const long head_bytes = kv4_head_bytes(bs, D), page_bytes = head_bytes * nkv;
@@ -181,21 +194,15 @@ __global__ __launch_bounds__(64 * NWV) __attribute__((amdgpu_waves_per_eu(2, 8))
     ask(UN);
   }
 
-  // ---- q of this lane's row: dims 64 s + 16 half .. and 64 s + 32 + 16 half .. of step s
+  // ---- q's two parts
   i32x8 qhi[KS], qlo[KS];
   float sl;
   {
-    const unsigned short* qp = static_cast<const unsigned short*>(a.q) + (long)(q0 + row) * a.q_stride + (long)h * D + 16 * half;
-    u16x8 raw[KS][4];
     unsigned am = 0;
 #pragma unroll
     for (int s = 0; s < KS; ++s)
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const int d0 = 64 * s + 32 * (e >> 1) + 8 * (e & 1);
-        raw[s][e] = d0 < D ? *reinterpret_cast<const u16x8*>(qp + d0) : u16x8{0, 0, 0, 0, 0, 0, 0, 0};
-        am = max(am, kv4_amax8(raw[s][e]));
-      }
+      for (int e = 0; e < 4; ++e) am = max(am, kv4_amax8(raw[s][e]));
     am = max(am, (unsigned)__shfl_xor((int)am, 32, 64));
     const int eb = min(max((int)(am >> 7), 16), 254);  // the largest value comes to [128, 256)
     const float down = __uint_as_float((unsigned)(eb - 7) << 23), down16 = __uint_as_float((unsigned)(eb - 11) << 23);
@@ -369,7 +376,7 @@ __global__ __launch_bounds__(64 * NWV) __attribute__((amdgpu_waves_per_eu(2, 8))
     int at = 0;
     for (int v = 0; v < nkt; v += UN) {
       const int next = UN - at;
-      if (early) {
+      if (early && v + UN < nkt) {
         put(next);
         fetch(v + 2 * UN);
         ask(v + 3 * UN);
@@ -377,7 +384,7 @@ __global__ __launch_bounds__(64 * NWV) __attribute__((amdgpu_waves_per_eu(2, 8))
 #pragma unroll 1
       for (int u = 0; u < UN; ++u)
         if (u == 0 || v + u < nkt) tile(v + u, buf[at + u]);
-      if (!early) {
+      if (!early && v + UN < nkt) {
         put(next);
         fetch(v + 2 * UN);
         ask(v + 3 * UN);
@@ -402,18 +409,24 @@ __global__ __launch_bounds__(64 * NWV) __attribute__((amdgpu_waves_per_eu(2, 8))
       if (live) scores(b0);
       __syncthreads();
       if (live) softmax(v, b0);
-      store(stage[0], b1);
-      store_scales(stage[0], b1);
-      fetch(v + 2);
-      ask(v + 3);
+      if (v + 1 < nkt) {
+        store(stage[0], b1);
+        store_scales(stage[0], b1);
+        fetch(v + 2);
+        ask(v + 3);
+      }
       __syncthreads();
     }
     if (live) values(nkt - 1, buf[(nkt - 1) & 1]);
   }
-  if (wrow0 + qi >= qlen) return;
+  // ---- rows through LDS, so that a row's dims leave together
+  __syncthreads();
+  if (wrow0 >= qlen) return;
   l_run = kv4_sum32(l_run);
   const float inv = l_run == 0.f ? 0.f : 1.f / l_run;  // a row that sees nothing: zeros
-  unsigned short* op = static_cast<unsigned short*>(a.out) + (long)(q0 + row) * a.out_stride + (long)h * D;
+  constexpr int OLD = D + 8;
+  static_assert(NWV * 32 * OLD * 2 <= 2 * UN * sizeof(Kv4Tile<D>), "the waves' rows fit the tiles' LDS");
+  unsigned short* ol = reinterpret_cast<unsigned short*>(smem) + wave * 32 * OLD;
 #pragma unroll
   for (int nb = 0; nb < NG; ++nb)
 #pragma unroll
@@ -421,8 +434,15 @@ __global__ __launch_bounds__(64 * NWV) __attribute__((amdgpu_waves_per_eu(2, 8))
       u16x4 w;
 #pragma unroll
       for (int j = 0; j < 4; ++j) w[j] = f32_to_bf16(o[nb][4 * g + j] * inv);
-      *reinterpret_cast<u16x4*>(op + 32 * nb + 8 * g + 4 * half) = w;
+      *reinterpret_cast<u16x4*>(ol + qi * OLD + 32 * nb + 8 * g + 4 * half) = w;
     }
+  unsigned short* op = static_cast<unsigned short*>(a.out) + (long)(q0 + wrow0) * a.out_stride + (long)h * D;
+#pragma unroll
+  for (int i = 0; i < 32 * D / 8; i += 64) {
+    const int r = (i + lane) / (D / 8), c = (i + lane) % (D / 8);
+    if (wrow0 + r < qlen)
+      *reinterpret_cast<u16x8*>(op + r * a.out_stride + 8 * c) = *reinterpret_cast<const u16x8*>(ol + r * OLD + 8 * c);
+  }
 }
 
 template <int D, int HG, int NWV>
