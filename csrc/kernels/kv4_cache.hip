@@ -8,7 +8,8 @@
 //
 // Bound by bytes for a prompt step and by the chain of loads for a decode step, hence two kernels: a token a workgroup, one
 // pass of loads for queries, key and value together; and runs of 16 tokens of a page, whose values leave as 16-byte stores (a
-// byte is one token's two dims, so single tokens store bytes).
+// byte is one token's two dims, so single tokens store bytes). Workgroups of a row's heads follow each other: rows of several heads are
+// neighbouring bytes (79000 rows read 140 us with the heads far apart).
 #include "hipserve/kv4.h"
 
 namespace hipserve {
@@ -93,7 +94,7 @@ __global__ __launch_bounds__(256) void kv4_write_token_kernel(unsigned short* __
                                                               int nkv, int bs) {
   constexpr int half = D / 2, CH = kMode == 0 ? half / 8 : D / 8;
   __shared__ __attribute__((aligned(16))) unsigned short kv[2][D];
-  const int t = blockIdx.x, kh = blockIdx.y;
+  const int t = blockIdx.x / nkv, kh = blockIdx.x % nkv;
   const int h0 = nq * kh / nkv, nh = nq * (kh + 1) / nkv - h0;  // this kv head's queries
   const long slot = slots[t];
   unsigned short* row = qkv + t * qkv_stride;
@@ -199,8 +200,8 @@ __global__ __launch_bounds__(256) void kv4_write_rows_kernel(unsigned short* __r
   __shared__ __attribute__((aligned(16))) unsigned short ks[16][D + PAD];
   __shared__ __attribute__((aligned(16))) unsigned char vcode[D / 2][16];
   __shared__ __attribute__((aligned(16))) unsigned char scale[2][NG][16];
-  const Kv4Rows rows = kv4_rows(slots, nslots, blockIdx.x * 16, T);
-  const int kh = blockIdx.y;
+  const Kv4Rows rows = kv4_rows(slots, nslots, blockIdx.x / nkv * 16, T);
+  const int kh = blockIdx.x % nkv;
   const int h0 = nq * kh / nkv, nh = nq * (kh + 1) / nkv - h0;  // this kv head's queries, then its key
   const int tt = threadIdx.x >> 4, l = threadIdx.x & 15, c = l % CH;
   const long head_bytes = kv4_head_bytes(bs, D);
@@ -294,7 +295,7 @@ static void kv4_write(unsigned short* q, long qkv_stride, const Kv4In& in, const
   const long nslots = c.blocks * c.block_size;
   if (in.ws == nullptr && T >= kKv4RowsFrom) {
 #define HS_KV4_WRITE(mode_)                                                                                              \
-  kv4_write_rows_kernel<mode_, D><<<dim3(cdiv(T, 16), c.nkv), 256, 0, s>>>(q, qkv_stride, positions, max_pos, slots, cos_sin, kc, \
+  kv4_write_rows_kernel<mode_, D><<<cdiv(T, 16) * c.nkv, 256, 0, s>>>(q, qkv_stride, positions, max_pos, slots, cos_sin, kc, \
                                                                            vc, nslots, T, nq, c.nkv, c.block_size)
     if (mode == 0) HS_KV4_WRITE(0);
     else HS_KV4_WRITE(1);
@@ -305,7 +306,7 @@ static void kv4_write(unsigned short* q, long qkv_stride, const Kv4In& in, const
   const int items = (cdiv(nq, c.nkv) + 1) * (mode == 0 ? D / 16 : D / 8) + D / 8;
   const int threads = min(256, cdiv(items, 64) * 64);
 #define HS_KV4_WRITE(mode_, parts)                                                                                        \
-  kv4_write_token_kernel<mode_, parts, D><<<dim3(T, c.nkv), threads, 0, s>>>(q, qkv_stride, in, positions, max_pos, slots, cos_sin, \
+  kv4_write_token_kernel<mode_, parts, D><<<T * c.nkv, threads, 0, s>>>(q, qkv_stride, in, positions, max_pos, slots, cos_sin, \
                                                                              kc, vc, nslots, nq, c.nkv, c.block_size)
   if (in.ws != nullptr) {
     if (mode == 0) HS_KV4_WRITE(0, true);
@@ -336,18 +337,21 @@ HS_DEVICE u32x4 kv4_widen8(unsigned w, int byte) {
   return u32x4{kv4_widen2<0>(w, s), kv4_widen2<1>(w, s), kv4_widen2<2>(w, s), kv4_widen2<3>(w, s)};
 }
 
-// Rows of slots as bf16: runs of 16 as the writer takes them, 16 lanes a token, 8 dims a lane. Bound by the bytes of the rows. A whole
-// run's value codes come as 16 tokens of a pair of dims and turn in LDS.
-template <int D>
+// Rows of slots as bf16: runs of 16 as the writer takes them, 16 lanes a token, 8 dims a lane, of kHeads heads. Bound by the bytes of
+// the rows where enough loads are under way: four heads a workgroup ask for theirs together. A whole run's value codes come as 16 tokens
+// of a pair of dims and turn in LDS.
+template <int D, int kHeads>
 __global__ __launch_bounds__(256) void kv4_read_kernel(unsigned short* __restrict__ k_out, long k_stride,
                                                        unsigned short* __restrict__ v_out, long v_stride,
                                                        const unsigned char* __restrict__ k_cache,
                                                        const unsigned char* __restrict__ v_cache,
                                                        const long* __restrict__ slots, long nslots, int T, int nkv, int bs) {
   constexpr int C8 = D / 8, ROW = D / 2 + 4;
-  __shared__ __attribute__((aligned(16))) unsigned char vcode[16][ROW];
-  const Kv4Rows rows = kv4_rows(slots, nslots, blockIdx.x * 16, T);
-  const int kh = blockIdx.y, tt = threadIdx.x >> 4, l = threadIdx.x & 15;
+  __shared__ __attribute__((aligned(16))) unsigned char vcode[kHeads][16][ROW];
+  const int parts = cdiv(nkv, kHeads);
+  const Kv4Rows rows = kv4_rows(slots, nslots, blockIdx.x / parts * 16, T);
+  const int kh0 = blockIdx.x % parts * kHeads, heads = min(kHeads, nkv - kh0);
+  const int tt = threadIdx.x >> 4, l = threadIdx.x & 15;
   const long head_bytes = kv4_head_bytes(bs, D);
   const int code_bytes = kv4_code_bytes(bs, D);
   for (int r0 = rows.first; r0 < rows.end; r0 += 16) {
@@ -355,32 +359,40 @@ __global__ __launch_bounds__(256) void kv4_read_kernel(unsigned short* __restric
     const long slot = rows.whole ? rows.slot + tt : t < rows.end ? slots[t] : -1;
     const bool keep = slot >= 0 && slot < nslots;
     const int off = keep ? (int)(slot % bs) : 0;
-    const long base = keep ? (slot / bs * nkv + kh) * head_bytes : 0;
-    const unsigned char *kp = k_cache + base, *vp = v_cache + base;
+    const long base = keep ? (slot / bs * nkv + kh0) * head_bytes : 0;
     if (rows.whole) {
-      const int i = threadIdx.x;
-      if (i < D / 2) {
-        const u32x4 w = *reinterpret_cast<const u32x4*>(v_cache + (rows.slot / bs * nkv + kh) * head_bytes + i * bs + rows.slot % bs);
+      const int u = threadIdx.x / (D / 2), i = threadIdx.x % (D / 2);
+      if (u < heads) {
+        const u32x4 w = *reinterpret_cast<const u32x4*>(v_cache + (rows.slot / bs * nkv + kh0 + u) * head_bytes + i * bs + rows.slot % bs);
 #pragma unroll
-        for (int j = 0; j < 16; ++j) vcode[j][i] = (unsigned char)(w[j >> 2] >> (8 * (j & 3)));
+        for (int j = 0; j < 16; ++j) vcode[u][j][i] = (unsigned char)(w[j >> 2] >> (8 * (j & 3)));
       }
-      __syncthreads();
     }
-    if (t < rows.end && l < C8) {
-      u32x4 ko{0, 0, 0, 0}, vo{0, 0, 0, 0};
-      if (keep) {
-        unsigned w = 0;
-        if (rows.whole) {
-          w = *reinterpret_cast<const unsigned*>(&vcode[tt][l * 4]);
-        } else {
+    const bool mine = t < rows.end && l < C8;
+    unsigned kc[kHeads], vc[kHeads];
+    int kb[kHeads], vb[kHeads];
 #pragma unroll
-          for (int j = 0; j < 4; ++j) w |= (unsigned)vp[(l * 4 + j) * bs + off] << (8 * j);
-        }
-        ko = kv4_widen8(*reinterpret_cast<const unsigned*>(kp + off * (D / 2) + l * 4), kp[code_bytes + (l >> 2) * bs + kv4_key_scale_at(off)]);
-        vo = kv4_widen8(w, vp[code_bytes + (l >> 2) * bs + off]);
-      }
-      __builtin_nontemporal_store(ko, reinterpret_cast<u32x4*>(k_out + t * k_stride + kh * D + l * 8));
-      __builtin_nontemporal_store(vo, reinterpret_cast<u32x4*>(v_out + t * v_stride + kh * D + l * 8));
+    for (int u = 0; u < kHeads; ++u) {
+      kc[u] = vc[u] = 0;
+      kb[u] = vb[u] = 127;  // a slot outside of the cache: zeros
+      if (!mine || !keep || u >= heads) continue;
+      const unsigned char *kp = k_cache + base + u * head_bytes, *vp = v_cache + base + u * head_bytes;
+      kc[u] = *reinterpret_cast<const unsigned*>(kp + off * (D / 2) + l * 4);
+      kb[u] = kp[code_bytes + (l >> 2) * bs + kv4_key_scale_at(off)];
+      vb[u] = vp[code_bytes + (l >> 2) * bs + off];
+      if (!rows.whole)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) vc[u] |= (unsigned)vp[(l * 4 + j) * bs + off] << (8 * j);
+    }
+    if (rows.whole) __syncthreads();
+    if (!mine) continue;
+#pragma unroll
+    for (int u = 0; u < kHeads; ++u) {
+      if (u >= heads) break;
+      if (rows.whole) vc[u] = *reinterpret_cast<const unsigned*>(&vcode[u][tt][l * 4]);
+      const long at = (long)(kh0 + u) * D + l * 8;
+      __builtin_nontemporal_store(kv4_widen8(kc[u], kb[u]), reinterpret_cast<u32x4*>(k_out + t * k_stride + at));
+      __builtin_nontemporal_store(kv4_widen8(vc[u], vb[u]), reinterpret_cast<u32x4*>(v_out + t * v_stride + at));
     }
   }
 }
@@ -388,15 +400,14 @@ __global__ __launch_bounds__(256) void kv4_read_kernel(unsigned short* __restric
 void launch_kv4_read(void* k_out, long k_stride, void* v_out, long v_stride, const Kv4Cache& c, const long* slots, int T,
                      hipStream_t s) {
   if (T <= 0) return;
-  const dim3 grid(cdiv(T, 16), c.nkv);
-#define HS_KV4_READ(d)                                                                                                    \
-  kv4_read_kernel<d><<<grid, 256, 0, s>>>(static_cast<unsigned short*>(k_out), k_stride, static_cast<unsigned short*>(v_out), \
-                                          v_stride, static_cast<const unsigned char*>(c.k),                               \
-                                          static_cast<const unsigned char*>(c.v), slots, c.blocks * c.block_size, T, c.nkv, \
-                                          c.block_size)
-  if (c.D == 128) HS_KV4_READ(128);
-  else if (c.D == 96) HS_KV4_READ(96);
-  else HS_KV4_READ(64);
+#define HS_KV4_READ(d, heads)                                                                                             \
+  kv4_read_kernel<d, heads><<<cdiv(T, 16) * cdiv(c.nkv, heads), 256, 0, s>>>(                                            \
+      static_cast<unsigned short*>(k_out), k_stride, static_cast<unsigned short*>(v_out), v_stride,                       \
+      static_cast<const unsigned char*>(c.k), static_cast<const unsigned char*>(c.v), slots, c.blocks * c.block_size, T,   \
+      c.nkv, c.block_size)
+  if (c.D == 128) HS_KV4_READ(128, 4);
+  else if (c.D == 96) HS_KV4_READ(96, 4);
+  else HS_KV4_READ(64, 4);
 #undef HS_KV4_READ
 }
 

@@ -275,6 +275,7 @@ static void kv4_write(at::Tensor& qkv, const at::Tensor* ws, int64_t splits, con
   const hipserve::Kv4Cache c = kv4_cache(k_cache, v_cache, nkv, who);
   TORCH_CHECK(c.D == head_dim, who, ": the cache holds heads of ", c.D);
   TORCH_CHECK(nq >= 0 && (mode == 0 || mode == 1), who, ": nq >= 0, mode 0 (rotate-half) or 1 (neighbouring dims)");
+  TORCH_CHECK(qkv.dim() == 2 && qkv.size(0) * nkv <= INT32_MAX, who, ": too many rows");
   const int64_t T = qkv.size(0), N = (nq + 2 * nkv) * head_dim;
   kv4_rows(qkv, k_cache, N, who, "qkv");
   const int64_t* pos = kv4_longs(positions, k_cache, T, who, "positions");
@@ -327,7 +328,7 @@ void read_cache_mx4(at::Tensor& k_out, at::Tensor& v_out, const at::Tensor& k_ca
                     (T <= 1 || o->stride(0) >= c.nkv * c.D) && o->stride(0) % 8 == 0 &&
                     reinterpret_cast<uintptr_t>(o->data_ptr()) % 16 == 0,
                 "read_cache: outputs are bf16 [rows, kv heads, head_dim], a row's heads together, rows at multiples of 16 bytes");
-  TORCH_CHECK(T < (1LL << 30), "read_cache: too many rows");
+  TORCH_CHECK(T * c.nkv <= INT32_MAX, "read_cache: too many rows");
   const int64_t* sl = kv4_longs(slots, k_cache, T, "read_cache", "slots");
   c10::hip::HIPGuardMasqueradingAsCUDA g(k_cache.device());
   hipserve::launch_kv4_read(k_out.data_ptr(), k_out.stride(0), v_out.data_ptr(), v_out.stride(0), c, sl, (int)T, cur_stream());

@@ -230,6 +230,49 @@ def test_write_holds_the_quantised_rows(dev, mode, nq, nkv, d, bs, t, order):
     assert torch.equal(kc.cpu(), want[0]) and torch.equal(vc.cpu(), want[1])
 
 
+@pytest.mark.parametrize("dev", DEVICES)
+@pytest.mark.parametrize("mode", [0, 1])
+@pytest.mark.parametrize("nq,nkv,d,bs", [(32, 8, 128, 16), (6, 6, 96, 32), (14, 2, 64, 256), (9, 3, 128, 64)])
+def test_write_and_read_of_ragged_prompts(dev, mode, nq, nkv, d, bs):
+    """A prompt step of many rows: sequences that begin anywhere in the step and in a page, single rows, whole pages, rows of no slot
+    between them, pages in any order. Written and read rows are the quantised rows of the same call on a bf16 cache."""
+    gen = torch.Generator().manual_seed(bs)
+    ops, lens = get_ops(dev), [(0, 70), (5, 6), (0, 1), (3, 100), (16, 48), (0, 131), (9, 10), (0, 16), (250, 300)]
+    nb = sum(-(-e // bs) for _, e in lens) + 4
+    pages = iter(torch.randperm(nb, generator=gen).tolist())
+    slots = []
+    for first, end in lens:
+        own = [next(pages) for _ in range(-(-end // bs))]
+        slots += [own[p // bs] * bs + p % bs for p in range(first, end)] + [-1] * (first % 2)
+    last = next(pages)
+    slots += [last * bs + o for o in (3, 1, 2, 0, 4)]      # backwards and forwards within a page
+    t = len(slots)
+    assert t > 300
+    slots = torch.tensor(slots).to(dev)
+    n = (nq + 2 * nkv) * d
+    x = _values(gen, t, n).to(dev)
+    pos, cs = torch.randint(0, 500, (t,), generator=gen).to(dev), ref.rope_cos_sin(d, 512, 10000.0).to(dev)
+    kb = torch.zeros(nb, nkv, bs, d, device=dev, dtype=torch.bfloat16)
+    vb = torch.zeros(nb, nkv, d, bs, device=dev, dtype=torch.bfloat16)
+    kc, vc = (c.to(dev) for c in _random_cache(gen, nb, nkv, bs, d))
+    want = [kc.cpu().clone(), vc.cpu().clone()]
+    plain, rows = x.clone(), x.clone()
+    ops.rope_cache(plain, pos, slots, cs, kb, vb, nq, nkv, d, mode)
+    ops.rope_cache(rows, pos, slots, cs, kc, vc, nq, nkv, d, mode)
+    assert torch.equal(rows[:, : nq * d], plain[:, : nq * d])
+    ok = slots >= 0
+    s = slots[ok]
+    held = kb[s // bs, :, s % bs].cpu(), vb[s // bs, :, :, s % bs].cpu()
+    for c, r, values in zip(want, held, (False, True)):
+        kv4.store(c, s.cpu(), r, values)
+    assert torch.equal(kc.cpu(), want[0]) and torch.equal(vc.cpu(), want[1])
+    k, v = (torch.full((t, nkv, d), 5.0, device=dev, dtype=torch.bfloat16) for _ in "kv")
+    ops.read_cache(k, v, kc, vc, slots)
+    for got, r in zip((k, v), held):
+        assert torch.equal(got[ok].cpu(), kv4.dequantise(*kv4.quantise(r)))
+        assert not got[~ok].any()
+
+
 @pytest.mark.gpu
 @pytest.mark.parametrize("t,splits", [(1, 1), (5, 3), (64, 8), (100, 17)])
 @pytest.mark.parametrize("extra", ["plain", "bias", "norm", "neighbours"])
