@@ -85,6 +85,20 @@ HS_DEVICE void kv4_split8(const u16x8 v, float scale, float scale16, u32x2& hi, 
   }
 }
 
+// Scale bytes of a query's two parts, hi in byte 0, lo in byte 1, from its largest magnitude's bits: that value comes to
+// [128, 256) of e4m3's 448. Of a query that holds a NaN or an infinity both are 255: its scores are NaN.
+HS_DEVICE int kv4_query_scales(unsigned amax_bits) {
+  if (amax_bits >= 0x7f80u) return 0xffff;
+  const int e = max((int)(amax_bits >> 7), 16);
+  return (e - 7) | (e - 11) << 8;
+}
+// scores to base 2; never 0, as a hidden key's -inf has to stay one
+HS_DEVICE float kv4_score_scale(float scale) { return fmaxf(scale * kLog2E, 1.17549435e-38f); }
+constexpr float kKv4Least = -3.4028235e38f;  // where a running maximum begins
+// exp2(score * scale - maximum) takes the product unrounded, the maximum is a rounded one: what is between them is a factor of the whole row,
+// and no more than 2 up to here. Rows beyond round their products first.
+HS_DEVICE bool kv4_far(float m) { return m != kKv4Least && fabsf(m) > 16777216.f; }
+
 // Blocks' ids of a sequence come from its block table. One outside of the cache is no page: its keys are not visible.
 HS_DEVICE int kv4_page(int id, long blocks) { return (unsigned)id < (unsigned long)blocks ? id : -1; }
 

@@ -181,7 +181,7 @@ HS_DEVICE Kv4Rows kv4_rows(const long* __restrict__ slots, long nslots, int t0, 
   r.end = min(t0 + e, T);
   r.slot = __builtin_bit_cast(long, ((unsigned long)(unsigned)__builtin_amdgcn_readlane((int)(s >> 32), f) << 32) |
                                         (unsigned)__builtin_amdgcn_readlane((int)s, f));
-  r.whole = r.end - r.first == 16 && ((mask >> f) & 0xffffu) == 1u && r.slot >= 0 && (r.slot & 15) == 0 && r.slot + 16 <= nslots;
+  r.whole = r.end - r.first == 16 && ((mask >> f) & 0xffffu) == 1u && r.slot >= 0 && (r.slot & 15) == 0 && r.slot <= nslots - 16;
   return r;
 }
 

@@ -7,7 +7,7 @@
 //  * scores: K codes go from memory into v_mfma_scale_f32_16x16x128_f8f6f4 as they are, rows = 16 tokens, their scale bytes as its
 //    block scales. The other operand is q in two e4m3 numbers: a bf16 value has 8 significant bits, e4m3 has 4, and what the first
 //    leaves is one e4m3 number again, so q is exact (values below 2^-14 of the row's largest within 2^-21 of it) where one number alone
-//    would lose half of its bits. One power of two per row keeps both in range and goes into the softmax's scale.
+//    would lose half of its bits. A power of two per row keeps both in range: the scale byte of that operand.
 //  * P . V: a byte of V is one token's two dims; v_cvt_scalef32_pk_bf16_fp4 applies the token's scale as it widens, two
 //    v_perm per pair of tokens sort the two dims. Scales ride in the exponent, so a shift makes one of a byte.
 //  * tokens of a 64-key chunk sit so that the lanes that get their scores are the lanes that feed their P: no exchange.
@@ -108,12 +108,12 @@ HS_DEVICE i32x8 kv4_pad(const u32x4 a, const u32x4 b) {
   return i32x8{(int)a[0], (int)a[1], (int)a[2], (int)a[3], (int)b[0], (int)b[1], (int)b[2], (int)b[3]};
 }
 
-template <int kByte>  // 16 tokens x 128 dims of FP4 under byte kByte of ks, times q's two parts
-HS_DEVICE f32x4 kv4_scores(const u32x4 k, unsigned ks, const i32x8 hi, const i32x8 lo) {
+template <int kByte>  // 16 tokens x 128 dims of FP4 under byte kByte of ks, times q's two parts under bytes 0 and 1 of qs
+HS_DEVICE f32x4 kv4_scores(const u32x4 k, unsigned ks, const i32x8 hi, const i32x8 lo, int qs) {
   const i32x8 a = kv4_pad(k, u32x4{0, 0, 0, 0});
   f32x4 s = {0.f, 0.f, 0.f, 0.f};
-  s = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(a, lo, s, 4, 0, kByte, (int)ks, 0, 123);
-  return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(a, hi, s, 4, 0, kByte, (int)ks, 0, 127);
+  s = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(a, lo, s, 4, 0, kByte, (int)ks, 1, qs);
+  return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(a, hi, s, 4, 0, kByte, (int)ks, 0, qs);
 }
 
 // bytes of a word whose bit in `keep` (bit i: byte i) is set, 127 (scale 1) for the others
@@ -222,7 +222,8 @@ __global__ __launch_bounds__(64 * kKv4Waves) __attribute__((amdgpu_waves_per_eu(
     pg = next;
   }
   i32x8 qhi[D == 64 ? 2 : 1], qlo[D == 64 ? 2 : 1];
-  float sl;
+  int qs;
+  const float sl = kv4_score_scale(a.scale);
   {
     unsigned am = 0;
 #pragma unroll
@@ -232,10 +233,8 @@ __global__ __launch_bounds__(64 * kKv4Waves) __attribute__((amdgpu_waves_per_eu(
         am = max(am, kv4_amax8(raw[h][e]));
     am = max(am, (unsigned)__shfl_xor((int)am, 16, 64));
     am = max(am, (unsigned)__shfl_xor((int)am, 32, 64));
-    const int eb = min(max((int)(am >> 7), 16), 254);  // the largest value comes to [128, 256)
-    const float down = __uint_as_float((unsigned)(eb - 7) << 23), down16 = __uint_as_float((unsigned)(eb - 11) << 23);
-    // never 0: a hidden key's -inf has to stay one
-    sl = am >= 0x7f80u ? NAN : fmaxf(a.scale * kLog2E * down, 1.17549435e-38f);
+    qs = kv4_query_scales(am);
+    const float down = kv4_scale(qs & 255), down16 = kv4_scale(qs >> 8 & 255);
     u32x4 hi[NH], lo[NH];
 #pragma unroll
     for (int h = 0; h < NH; ++h)
@@ -263,7 +262,8 @@ __global__ __launch_bounds__(64 * kKv4Waves) __attribute__((amdgpu_waves_per_eu(
   f32x4 o[NG][2];  // rows: heads 4 grp + r, columns: dims 32 n + 2 col (+ 1)
 #pragma unroll
   for (int n = 0; n < NG; ++n) o[n][0] = o[n][1] = f32x4{0.f, 0.f, 0.f, 0.f};
-  float m_run = -1e30f, l_run = 0.f;  // of head `col`; the sum over this lane's tokens alone
+  float m_run = kKv4Least, l_run = 0.f;      // of head `col`; the sum over this lane's tokens alone
+  bool far = false;                          // of some head of the wave
 
   auto compute = [&](int c, Chunk& ch) {
     const int tok = chunks.token(c);
@@ -272,16 +272,16 @@ __global__ __launch_bounds__(64 * kKv4Waves) __attribute__((amdgpu_waves_per_eu(
     if constexpr (D == 64) {
       const unsigned sh = ch.ks >> (8 * (grp >> 1));  // bytes 0 and 2: this lane's tokens of the two loads
       const unsigned s0 = grp < 2 ? sh : 0x7f7f7f7fu, s1 = grp < 2 ? 0x7f7f7f7fu : sh;
-      st[0] = kv4_scores<0>(ch.k[0], s0, qhi[0], qlo[0]);
-      st[1] = kv4_scores<0>(ch.k[0], s1, qhi[1], qlo[1]);
-      st[2] = kv4_scores<2>(ch.k[1], s0, qhi[0], qlo[0]);
-      st[3] = kv4_scores<2>(ch.k[1], s1, qhi[1], qlo[1]);
+      st[0] = kv4_scores<0>(ch.k[0], s0, qhi[0], qlo[0], qs);
+      st[1] = kv4_scores<0>(ch.k[0], s1, qhi[1], qlo[1], qs);
+      st[2] = kv4_scores<2>(ch.k[1], s0, qhi[0], qlo[0], qs);
+      st[3] = kv4_scores<2>(ch.k[1], s1, qhi[1], qlo[1], qs);
     } else {
       const unsigned ks = D == 96 && grp == 3 ? 0x7f7f7f7fu : ch.ks;
-      st[0] = kv4_scores<0>(ch.k[0], ks, qhi[0], qlo[0]);
-      st[1] = kv4_scores<1>(ch.k[1], ks, qhi[0], qlo[0]);
-      st[2] = kv4_scores<2>(ch.k[2], ks, qhi[0], qlo[0]);
-      st[3] = kv4_scores<3>(ch.k[3], ks, qhi[0], qlo[0]);
+      st[0] = kv4_scores<0>(ch.k[0], ks, qhi[0], qlo[0], qs);
+      st[1] = kv4_scores<1>(ch.k[1], ks, qhi[0], qlo[0], qs);
+      st[2] = kv4_scores<2>(ch.k[2], ks, qhi[0], qlo[0], qs);
+      st[3] = kv4_scores<3>(ch.k[3], ks, qhi[0], qlo[0], qs);
     }
     const bool whole = tok + kKv4Chunk <= ctx && (tok >= chunks.lo || tok + kKv4Chunk <= a.sinks);
     if (!whole || __any(ch.page < 0)) {
@@ -306,6 +306,7 @@ __global__ __launch_bounds__(64 * kKv4Waves) __attribute__((amdgpu_waves_per_eu(
       const float m_new = fmaxf(m_run, mx);
       const float alpha = __builtin_amdgcn_exp2f(m_run - m_new);
       m_run = m_new;
+      far = __any(kv4_far(m_run));
       l_run *= alpha;
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
@@ -317,11 +318,17 @@ __global__ __launch_bounds__(64 * kKv4Waves) __attribute__((amdgpu_waves_per_eu(
         }
       }
     }
+    float by = sl;
+    if (far) {
+#pragma unroll
+      for (int i = 0; i < 16; ++i) st[i >> 2][i & 3] *= sl;
+      by = 1.f;
+    }
     float ps[4] = {0.f, 0.f, 0.f, 0.f};
     bf16x8 p[2];
 #pragma unroll
     for (int i = 0; i < 16; ++i) {
-      const float x = __builtin_amdgcn_exp2f(__builtin_fmaf(st[i >> 2][i & 3], sl, -m_run));
+      const float x = __builtin_amdgcn_exp2f(__builtin_fmaf(st[i >> 2][i & 3], by, -m_run));
       ps[i & 3] += x;
       p[i >> 3][i & 7] = static_cast<__bf16>(x);
     }
@@ -384,7 +391,7 @@ __global__ __launch_bounds__(64 * kKv4Waves) __attribute__((amdgpu_waves_per_eu(
   const bool one = chunks.count <= part_chunks;
   for (int i = tid; i < G * D; i += 64 * W) {
     const int h = i / D, d = i % D;
-    float M = -1e30f;
+    float M = kKv4Least;
 #pragma unroll
     for (int w = 0; w < W; ++w) M = fmaxf(M, red[(w * G + h) * 2]);
     float L = 0.f, acc = 0.f;
@@ -424,7 +431,7 @@ __global__ __launch_bounds__(256) void kv4_decode_merge_kernel(Kv4Attn a, const 
   if (count <= run.chunks) return;
   const int np = (count + run.chunks - 1) / run.chunks;
   const long base = ((long)b * a.nq + h) * max_parts;
-  float M = -1e30f;
+  float M = kKv4Least;
   for (int p = tid & 63; p < np; p += 64) M = fmaxf(M, tmp_ml[(base + p) * 2]);
   M = wave_max(M);
   float L[4] = {0.f, 0.f, 0.f, 0.f};

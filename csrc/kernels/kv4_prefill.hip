@@ -2,19 +2,31 @@
 // that stay visible beside it. Keys of the step itself come from the cache like the older ones: kv4_write has run before.
 //
 // Bound by the matrix cores and by what stands beside their products, so a tile is unpacked once for all its readers:
-//  * workgroup = up to 8 query heads of one kv head x blocks of 32 rows, a wave each; 64 keys a tile, staged through registers. Of 8
-//    waves the two on a SIMD are half a tile apart: one in its products (the scores of a tile, the values of the one before), the
-//    other in its softmax and staging, with a barrier between the halves (8192 rows 592 -> 564 us). Staging is then two
-//    tiles ahead, in four buffers. Workgroups of 4 waves come two a compute unit instead.
+//  * workgroup = up to 8 query heads of one kv head x blocks of 32 rows, a wave each; 64 keys a tile, staged through registers into
+//    the tiles of LDS after the ones in use.
+//    - 8 waves (two queries per kv head or more): two tiles a barrier, and half of the waves stage the next two before their products,
+//      the others after them: of a SIMD's two waves one unpacks while the other multiplies.
+//    - 4 waves (one query per kv head): the values of a tile and the scores of the next one together, one tile a barrier, two
+//      workgroups a compute unit, as four tiles of LDS would leave room for one.
+//    Each at the other's shape is slower: 8 waves by the second 887 against 840 us (4096 rows at 16384, 32 / 8 heads), 4 waves by
+//    the first 124 against 111 us (8 x 1024 rows, 32 / 32 heads).
 //  * S^T = K . Q^T on v_mfma_scale_f32_32x32x64_f8f6f4: K's codes lie in LDS as they are (a quarter of bf16's LDS reads), their
 //    scale bytes are the product's; q as two e4m3 numbers (see kv4_decode.hip), exact for a bf16 q, at bf16's rate.
 //  * V is widened to bf16 on its way into LDS, transposed as it lies in the cache: a thread takes 8 tokens of two dims, v_cvt applies the
 //    scales, v_perm sorts the dims.
 //  * keys sit in K's LDS rows with bits 2 and 3 exchanged: a lane's scores are then 8 neighbouring keys a step of the second product,
 //    O^T = V^T . P^T, and P is its operand without an exchange.
-//  * softmax in base 2, 32 bits; P is rounded to bf16, its sum is not; O is rescaled when a score is over 2^8 above the maximum.
+//  * softmax in base 2, 32 bits; P is rounded to bf16, as its product takes it, and its 32-bit sum is that of the rounded P: both come
+//    from one dot product instruction, and what the rounding does to the weights it does to their sum. O is rescaled when a
+//    score is over 2^8 above the maximum.
+//  * rows leave through LDS, a row's dims together: 16-byte stores of 256 neighbouring bytes.
 // Hidden keys have score -inf whatever they hold. A value's NaN (scale byte 255) must reach the rows that see it alone, and 0 * NaN is
 // not 0: it is staged as a finite number and put into the accumulators of the rows that see it, in a branch that no other tile takes.
+//
+// 32 / 8 heads of 128 dims: 8192 rows 543 us (1.01 PFLOP/s), 4096 rows at 16384 825 us (1.16), a window of 4096 there 269 us; the 8-bit
+// part of the products is twice the bf16 part's operations, so this is what a bf16 cache's kernel does (530, 876, 276 us) at 17 / 64 of its bytes.
+#include <atomic>
+
 #include "hipserve/kv4.h"
 
 namespace hipserve {
@@ -31,6 +43,8 @@ HS_DEVICE float kv4_sum32(float v) {
   const auto r = __builtin_amdgcn_permlane32_swap(u, u, false, false);
   return __builtin_bit_cast(float, (unsigned)r[0]) + __builtin_bit_cast(float, (unsigned)r[1]);
 }
+
+HS_DEVICE i32x8 kv4_pad(const u32x4 a) { return i32x8{(int)a[0], (int)a[1], (int)a[2], (int)a[3], 0, 0, 0, 0}; }
 
 // whether a byte of w is 255
 HS_DEVICE bool kv4_any_nan(unsigned w) { return (((w & 0x7f7f7f7fu) + 0x01010101u) & w & 0x80808080u) != 0; }
@@ -49,7 +63,7 @@ struct Kv4Tile {
   unsigned char nopage[4];                                          // runs of 16 tokens without a page
 };
 
-// kTwo: the two waves of a SIMD are half a tile apart (see above); else every wave is at the same step
+// HG: query heads a workgroup; NWV: its waves; UN: tiles a barrier
 template <int D, int HG, int NWV, int UN>
 __global__ __launch_bounds__(64 * NWV) __attribute__((amdgpu_waves_per_eu(2, 8))) void kv4_prefill_kernel(
     Kv4Attn a, const int* __restrict__ cu_q, int seqs, const int* __restrict__ ctx_lens, int rows,
@@ -196,7 +210,8 @@ __global__ __launch_bounds__(64 * NWV) __attribute__((amdgpu_waves_per_eu(2, 8))
 
   // ---- q's two parts
   i32x8 qhi[KS], qlo[KS];
-  float sl;
+  int qs;
+  const float sl = kv4_score_scale(a.scale);
   {
     unsigned am = 0;
 #pragma unroll
@@ -204,10 +219,8 @@ __global__ __launch_bounds__(64 * NWV) __attribute__((amdgpu_waves_per_eu(2, 8))
 #pragma unroll
       for (int e = 0; e < 4; ++e) am = max(am, kv4_amax8(raw[s][e]));
     am = max(am, (unsigned)__shfl_xor((int)am, 32, 64));
-    const int eb = min(max((int)(am >> 7), 16), 254);  // the largest value comes to [128, 256)
-    const float down = __uint_as_float((unsigned)(eb - 7) << 23), down16 = __uint_as_float((unsigned)(eb - 11) << 23);
-    // never 0: a hidden key's -inf has to stay one
-    sl = am >= 0x7f80u ? NAN : fmaxf(a.scale * kLog2E * down, 1.17549435e-38f);
+    qs = kv4_query_scales(am);
+    const float down = kv4_scale(qs & 255), down16 = kv4_scale(qs >> 8 & 255);
 #pragma unroll
     for (int s = 0; s < KS; ++s)
 #pragma unroll
@@ -227,7 +240,8 @@ __global__ __launch_bounds__(64 * NWV) __attribute__((amdgpu_waves_per_eu(2, 8))
   for (int nb = 0; nb < NG; ++nb)
 #pragma unroll
     for (int r = 0; r < 16; ++r) o[nb][r] = 0.f;
-  float m_run = -1e30f, l_run = 0.f;
+  float m_run = kKv4Least, l_run = 0.f;
+  bool far = false;  // of some row of the wave
 
   auto sees_some = [&](int v) {  // whether a row of the wave may see a key of tile v
     const int key = tile_key(v);
@@ -253,12 +267,11 @@ __global__ __launch_bounds__(64 * NWV) __attribute__((amdgpu_waves_per_eu(2, 8))
         if (D == 96 && s == 1 && half) ks[h2] = 127;  // no such dims: q is zero there, whatever the scale of others is
       }
 #pragma unroll
-      for (int part = 0; part < 2; ++part)
+      for (int h2 = 0; h2 < 2; ++h2)
+        st[h2] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(kv4_pad(kf[h2]), qlo[s], st[h2], 4, 0, 0, ks[h2], 1, qs);
 #pragma unroll
-        for (int h2 = 0; h2 < 2; ++h2)
-          st[h2] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(
-              i32x8{(int)kf[h2][0], (int)kf[h2][1], (int)kf[h2][2], (int)kf[h2][3], 0, 0, 0, 0},
-              part == 0 ? qlo[s] : qhi[s], st[h2], 4, 0, 0, ks[h2], 0, part == 0 ? 123 : 127);
+      for (int h2 = 0; h2 < 2; ++h2)
+        st[h2] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(kv4_pad(kf[h2]), qhi[s], st[h2], 4, 0, 0, ks[h2], 0, qs);
     }
   };
   auto softmax = [&](int v, const Kv4Tile<D>& b) __attribute__((always_inline)) {
@@ -303,19 +316,28 @@ __global__ __launch_bounds__(64 * NWV) __attribute__((amdgpu_waves_per_eu(2, 8))
       const float m_new = fmaxf(m_run, kv4_max32(mx));
       const float alpha = __builtin_amdgcn_exp2f(m_run - m_new);
       m_run = m_new;
+      far = __any(kv4_far(m_run));
       l_run *= alpha;
 #pragma unroll
       for (int nb = 0; nb < NG; ++nb)
 #pragma unroll
         for (int r = 0; r < 16; ++r) o[nb][r] *= alpha;
     }
+    float by = sl;
+    if (far) {
+#pragma unroll
+      for (int h2 = 0; h2 < 2; ++h2)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) st[h2][r] *= sl;
+      by = 1.f;
+    }
     // the sum is that of the rounded P, two at a time
     float ps[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
     for (int i = 0; i < 32; i += 2) {
       const f32x16& x = st[i >> 4];
-      const bf16x2 p{static_cast<__bf16>(__builtin_amdgcn_exp2f(__builtin_fmaf(x[i & 15], sl, -m_run))),
-                     static_cast<__bf16>(__builtin_amdgcn_exp2f(__builtin_fmaf(x[(i & 15) + 1], sl, -m_run)))};
+      const bf16x2 p{static_cast<__bf16>(__builtin_amdgcn_exp2f(__builtin_fmaf(x[i & 15], by, -m_run))),
+                     static_cast<__bf16>(__builtin_amdgcn_exp2f(__builtin_fmaf(x[(i & 15) + 1], by, -m_run)))};
       ps[(i >> 1) & 3] = __builtin_amdgcn_fdot2_f32_bf16(p, bf16x2{static_cast<__bf16>(1.f), static_cast<__bf16>(1.f)}, ps[(i >> 1) & 3], false);
       pb[i >> 3][i & 7] = p[0];
       pb[i >> 3][(i & 7) + 1] = p[1];
@@ -436,6 +458,8 @@ __global__ __launch_bounds__(64 * NWV) __attribute__((amdgpu_waves_per_eu(2, 8))
       for (int j = 0; j < 4; ++j) w[j] = f32_to_bf16(o[nb][4 * g + j] * inv);
       *reinterpret_cast<u16x4*>(ol + qi * OLD + 32 * nb + 8 * g + 4 * half) = w;
     }
+  __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");  // other lanes read what this one wrote
+  __builtin_amdgcn_wave_barrier();
   unsigned short* op = static_cast<unsigned short*>(a.out) + (long)(q0 + wrow0) * a.out_stride + (long)h * D;
 #pragma unroll
   for (int i = 0; i < 32 * D / 8; i += 64) {
@@ -451,9 +475,16 @@ static void kv4_prefill(const Kv4Attn& a, const int* cu_q, int seqs, const int* 
   constexpr int SUB = 128 / (32 * (NWV / HG));
   constexpr int UN = NWV == 8 ? 2 : 1;  // workgroups of 4 waves come two a compute unit
   constexpr int kLds = 2 * UN * sizeof(Kv4Tile<D>);
-  static const bool attr [[maybe_unused]] =
-      hipFuncSetAttribute(reinterpret_cast<const void*>(&kv4_prefill_kernel<D, HG, NWV, UN>),
-                          hipFuncAttributeMaxDynamicSharedMemorySize, kLds) == hipSuccess;
+  if (kLds > 64 * 1024) {  // more than the default limit: asked for once a device
+    static std::atomic<unsigned long> asked{0};
+    int dev = 0;
+    (void)hipGetDevice(&dev);
+    const unsigned long bit = 1ul << (dev & 63);
+    if ((asked.load(std::memory_order_relaxed) & bit) == 0 &&
+        hipFuncSetAttribute(reinterpret_cast<const void*>(&kv4_prefill_kernel<D, HG, NWV, UN>),
+                            hipFuncAttributeMaxDynamicSharedMemorySize, kLds) == hipSuccess)
+      asked.fetch_or(bit, std::memory_order_relaxed);
+  }
   kv4_prefill_kernel<D, HG, NWV, UN><<<dim3(ntiles * SUB, a.nq / HG), 64 * NWV, kLds, s>>>(a, cu_q, seqs, ctx, rows, tiles);
 }
 

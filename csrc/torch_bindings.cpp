@@ -243,6 +243,8 @@ static hipserve::Kv4Cache kv4_cache(const at::Tensor& k, const at::Tensor& v, in
                   k.is_contiguous() && v.is_contiguous() && k.is_cuda() && v.device() == k.device(),
               who, ": mxfp4 caches are contiguous uint8 [blocks, kv heads, block_size, 17 head_dim / 32], K and V alike");
   TORCH_CHECK(nkv > 0 && k.size(1) == nkv, who, ": the cache has ", k.size(1), " kv heads, not ", nkv);
+  TORCH_CHECK(reinterpret_cast<uintptr_t>(k.data_ptr()) % 16 == 0 && reinterpret_cast<uintptr_t>(v.data_ptr()) % 16 == 0, who,
+              ": caches start at a multiple of 16 bytes");
   const int64_t w = k.size(3), bs = k.size(2), D = w * 32 / 17;
   TORCH_CHECK(w % 17 == 0 && (D == 64 || D == 96 || D == 128), who, ": head_dim 64, 96 or 128");
   TORCH_CHECK(bs >= 16 && bs <= 256 && (bs & (bs - 1)) == 0, who, ": block_size a power of two in [16, 256]");
@@ -275,7 +277,8 @@ static void kv4_write(at::Tensor& qkv, const at::Tensor* ws, int64_t splits, con
   const hipserve::Kv4Cache c = kv4_cache(k_cache, v_cache, nkv, who);
   TORCH_CHECK(c.D == head_dim, who, ": the cache holds heads of ", c.D);
   TORCH_CHECK(nq >= 0 && (mode == 0 || mode == 1), who, ": nq >= 0, mode 0 (rotate-half) or 1 (neighbouring dims)");
-  TORCH_CHECK(qkv.dim() == 2 && qkv.size(0) * nkv <= INT32_MAX, who, ": too many rows");
+  // workgroups of 256 threads: a row and kv head each, or 16 rows
+  TORCH_CHECK(qkv.dim() == 2 && qkv.size(0) * nkv < (ws != nullptr ? 1 << 24 : 1 << 28), who, ": too many rows");
   const int64_t T = qkv.size(0), N = (nq + 2 * nkv) * head_dim;
   kv4_rows(qkv, k_cache, N, who, "qkv");
   const int64_t* pos = kv4_longs(positions, k_cache, T, who, "positions");
@@ -285,7 +288,7 @@ static void kv4_write(at::Tensor& qkv, const at::Tensor* ws, int64_t splits, con
               who, ": cos_sin fp32 [positions, head_dim]");
   if (ws != nullptr)
     TORCH_CHECK(ws->device() == k_cache.device() && ws->scalar_type() == at::kFloat && ws->is_contiguous() && splits > 0 &&
-                    ws->numel() >= splits * T * N,
+                    ws->numel() >= splits * T * N && reinterpret_cast<uintptr_t>(ws->data_ptr()) % 16 == 0,
                 who, ": fp32 partials [splits, rows, (nq + 2 nkv) head_dim]");
   if (bias != nullptr)
     TORCH_CHECK(bias->device() == k_cache.device() && bias->scalar_type() == at::kBFloat16 && bias->is_contiguous() &&
@@ -328,7 +331,7 @@ void read_cache_mx4(at::Tensor& k_out, at::Tensor& v_out, const at::Tensor& k_ca
                     (T <= 1 || o->stride(0) >= c.nkv * c.D) && o->stride(0) % 8 == 0 &&
                     reinterpret_cast<uintptr_t>(o->data_ptr()) % 16 == 0,
                 "read_cache: outputs are bf16 [rows, kv heads, head_dim], a row's heads together, rows at multiples of 16 bytes");
-  TORCH_CHECK(T * c.nkv <= INT32_MAX, "read_cache: too many rows");
+  TORCH_CHECK(T * c.nkv < 1 << 28, "read_cache: too many rows");
   const int64_t* sl = kv4_longs(slots, k_cache, T, "read_cache", "slots");
   c10::hip::HIPGuardMasqueradingAsCUDA g(k_cache.device());
   hipserve::launch_kv4_read(k_out.data_ptr(), k_out.stride(0), v_out.data_ptr(), v_out.stride(0), c, sl, (int)T, cur_stream());
@@ -346,7 +349,7 @@ static hipserve::Kv4Attn kv4_attn(at::Tensor& out, const at::Tensor& q, const at
   TORCH_CHECK(block_tables.device() == k_cache.device() && block_tables.scalar_type() == at::kInt && block_tables.dim() == 2 &&
                   block_tables.stride(1) == 1 && block_tables.stride(0) <= INT32_MAX,
               who, ": block tables int32 [sequences, blocks]");
-  TORCH_CHECK(block_tables.size(1) * a.cache.block_size <= INT32_MAX - 1024, who, ": contexts of up to 2^31 tokens");
+  TORCH_CHECK(block_tables.size(1) * a.cache.block_size <= 1 << 30, who, ": contexts of up to 2^30 tokens");
   a.out = out.data_ptr();
   a.out_stride = out.stride(0);
   a.q = q.data_ptr();
@@ -356,8 +359,9 @@ static hipserve::Kv4Attn kv4_attn(at::Tensor& out, const at::Tensor& q, const at
   a.bt_width = block_tables.size(1);
   a.nq = nq;
   a.scale = (float)scale;
-  a.window = window;
-  a.sinks = window > 0 ? sinks : 0;  // without a window every key is visible
+  // sums and differences with them stay in 32 bits; wider ones show no other keys
+  a.window = std::min<int64_t>(window, 1 << 30);
+  a.sinks = window > 0 ? std::min<int64_t>(sinks, 1 << 30) : 0;  // without a window every key is visible
   return a;
 }
 void paged_decode_mx4(at::Tensor& out, const at::Tensor& q, const at::Tensor& k_cache, const at::Tensor& v_cache,
@@ -372,7 +376,7 @@ void paged_decode_mx4(at::Tensor& out, const at::Tensor& q, const at::Tensor& k_
   for (const at::Tensor* t : {&tmp_out, &tmp_ml})
     TORCH_CHECK(t->device() == k_cache.device() && t->scalar_type() == at::kFloat && t->is_contiguous() && t->dim() == 4 &&
                     t->size(0) >= B && t->size(1) == nq && t->size(2) == tmp_ml.size(2) && t->size(2) > 0 &&
-                    t->size(3) == (t == &tmp_ml ? 2 : a.cache.D),
+                    t->size(3) == (t == &tmp_ml ? 2 : a.cache.D) && reinterpret_cast<uintptr_t>(t->data_ptr()) % 16 == 0,
                 "paged_decode: workspaces fp32 [rows, nq, partitions, head_dim] and [rows, nq, partitions, 2]");
   TORCH_CHECK(tmp_ml.size(2) * part_size >= block_tables.size(1) * a.cache.block_size,
               "workspace partitions must cover block_tables capacity");
@@ -386,7 +390,8 @@ void prefill_attention_mx4(at::Tensor& out, const at::Tensor& q, const at::Tenso
   const hipserve::Kv4Attn a = kv4_attn(out, q, k_cache, v_cache, block_tables, nq, nkv, scale, window, sinks, "prefill_attention");
   const int64_t seqs = cu_q.numel() - 1;
   TORCH_CHECK(seqs >= 0 && block_tables.size(0) >= seqs, "prefill_attention: a block table per sequence");
-  TORCH_CHECK(tiles.dim() == 2 && tiles.size(1) == 2, "prefill_attention: tiles [tiles, 2]");
+  TORCH_CHECK(tiles.dim() == 2 && tiles.size(1) == 2 && tiles.size(0) <= 1 << 20 && tiles.size(0) * nq <= INT32_MAX,
+              "prefill_attention: tiles [tiles, 2], at most 2^20 and 2^31 over the heads");
   const int* cu = kv4_ints(cu_q, k_cache, 1, "prefill_attention", "row offsets");
   const int* ctx = kv4_ints(ctx_lens, k_cache, seqs, "prefill_attention", "context lengths");
   const int* tl = kv4_ints(tiles, k_cache, 0, "prefill_attention", "tiles");

@@ -119,6 +119,9 @@ class ModelRunner:
             if not getattr(self.model, "supports_mxfp4_kv", False):
                 raise ValueError(f"{mcfg.name}: this model has no mxfp4 KV cache")
             kv4.cache_shape(1, 1, self.block_size, self.model.D)  # refuses a head size that the cache does not hold
+            if self.model.nq > 16 * self.model.nkv:
+                raise ValueError(f"{mcfg.name}: the mxfp4 KV cache serves up to 16 queries per kv head, not "
+                                 f"{self.model.nq // self.model.nkv}")
             self.model.kv_dtype = kv4.DTYPE
             self.model.fused_qkv_attention = False
             self.model.attention_sinks = ecfg.attention_sinks

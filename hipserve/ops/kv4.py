@@ -152,12 +152,12 @@ def sees(pos, tokens, window: int, sinks: int):
 
 
 def paged_decode(q, k_cache, v_cache, block_tables, context_lens, nq, nkv, scale, window=0, sinks=0):
-    """q [B, nq * D (+ extra)] -> [B, nq, D]."""
+    """q [B, nq * D (+ extra)] -> [B, nq, D]. A length beyond the block table's tokens counts as those."""
     check(k_cache, v_cache, nkv)
     D = head_dim(k_cache)
     out = torch.empty(q.shape[0], nq, D, dtype=q.dtype, device=q.device)
     for b in range(q.shape[0]):
-        n = max(0, int(context_lens[b]))
+        n = max(0, min(int(context_lens[b]), block_tables.shape[1] * k_cache.shape[2]))
         k, v, ok = context(k_cache, v_cache, block_tables[b], n)
         seen = sees(torch.tensor([n - 1], device=q.device), k.shape[0], window, sinks) & ok
         out[b] = attend(q[b:b + 1, : nq * D].view(1, nq, D), k, v, seen, scale)[0].to(q.dtype)

@@ -76,7 +76,8 @@ def _oracle(q, kc, vc, tables, rows, ctx, nq, nkv, scale, window, sinks):
 
 
 def _check(got, want, size):
-    """A probability is rounded to bf16 once and the output once: 2^-8 of each. Scores are sums of 32 bits of up to 128 products of a few
+    """A probability is rounded to bf16 once and the output once: 2^-8 of each (a prompt's sum is that of the rounded probabilities, which
+    allows another 2^-8 of the output; held to the same). Scores are sums of 32 bits of up to 128 products of a few
     units, off by under 2^-14 in the exponent, and the sums over the keys add less: together under 2^-11 of the sum of p |v|."""
     got = got.float().cpu().double().view(want.shape)
     assert torch.equal(got.isnan(), want.isnan())
@@ -493,6 +494,80 @@ def _check_sharp(got, want, size):
     assert (off <= (2 ** -8 + 2 ** -7) * 2 * size + 2 ** -8 * want.abs() + 1e-30).all()
 
 
+@pytest.mark.parametrize("dev", DEVICES)
+@pytest.mark.parametrize("window,sinks", [(2 ** 31 - 1, 0), (2 ** 31 - 1, 2 ** 31 - 1), (1, 2 ** 31 - 1), (100, 150), (2 ** 30, 5)])
+def test_the_widest_windows(dev, window, sinks):
+    """A window or first tokens beyond every context: all keys up to a row's own are seen."""
+    gen = torch.Generator().manual_seed(21)
+    nq, nkv, d, bs, ctx = 8, 2, 128, 16, [1, 150, 97]
+    nb, bt = _tables(gen, ctx, bs)
+    kc, vc = _random_cache(gen, nb, nkv, bs, d)
+    rows = [1, 150, 40]
+    q = _queries(gen, sum(rows), nq, nkv, d)
+    want, size = _oracle(q, kc, vc, bt, rows, ctx, nq, nkv, 1 / math.sqrt(d), 0, 0)
+    _check(_prompt(get_ops(dev), dev, q, kc, vc, bt, rows, ctx, nq, nkv, d, window, sinks), want, size)
+    want, size = _oracle(q[:3], kc, vc, bt, [1] * 3, ctx, nq, nkv, 1 / math.sqrt(d), 0, 0)
+    for part in (64, 256):
+        _check(_decode(get_ops(dev), dev, q[:3], kc, vc, bt, ctx, nq, nkv, d, bs, part, window, sinks), want, size)
+
+
+@pytest.mark.parametrize("dev", DEVICES)
+def test_a_length_beyond_the_table_ends_with_it(dev):
+    """Decode: with a window too, the last keys are the table's last ones."""
+    gen = torch.Generator().manual_seed(22)
+    nq, nkv, d, bs, n = 8, 2, 128, 16, 160
+    nb, bt = _tables(gen, [n, n], bs)
+    kc, vc = _random_cache(gen, nb, nkv, bs, d)
+    q = _queries(gen, 2, nq, nkv, d)
+    want, size = _oracle(q, kc, vc, bt, [1, 1], [n, n], nq, nkv, 1 / math.sqrt(d), 50, 4)
+    _check(_decode(get_ops(dev), dev, q, kc, vc, bt, [2 ** 31 - 1, n + 30], nq, nkv, d, bs, 64, 50, 4), want, size)
+
+
+@pytest.mark.parametrize("dev", DEVICES)
+@pytest.mark.parametrize("d", [64, 96, 128])
+def test_scores_at_the_ends_of_the_range(dev, d):
+    """Scores around -2^110 (one product each, so exact): the least negative one takes all, wherever it stands; the others' weights are 0,
+    so the output is that value within its own rounding, of which a 4-bit value has none."""
+    gen = torch.Generator().manual_seed(23)
+    nq, nkv, bs, n = 8, 2, 16, 300
+    nb, bt = _tables(gen, [n, n], bs)
+    kc, vc = _random_cache(gen, nb, nkv, bs, d)
+    kc.view(nb, nkv, -1)[..., : bs * d // 2] = 0
+    kc.view(nb, nkv, -1)[..., bs * d // 2:] = 127 + 50
+    for b in range(nb):   # dim 0 of every key: -6, of token 211: -4
+        for t in range(bs):
+            kc.view(nb, nkv, -1)[b, :, t * d // 2] = 15
+    kc.view(nb, nkv, -1)[int(bt[0, 211 // bs]), :, 211 % bs * d // 2] = 14
+    kc.view(nb, nkv, -1)[int(bt[1, 211 // bs]), :, 211 % bs * d // 2] = 14
+    q = torch.zeros(600, (nq + 2 * nkv) * d, dtype=torch.bfloat16)
+    q[:, ::d] = 2.0 ** 60
+    vals = _decode_bytes(vc, True)
+    one = torch.stack([vals[int(bt[i, 211 // bs]), :, 211 % bs] for i in (0, 1)]).repeat_interleave(nq // nkv, 1)  # [2, nq, d]
+    for part in (64, 512):
+        got = _decode(get_ops(dev), dev, q[:2], kc, vc, bt, [n, n], nq, nkv, d, bs, part, 0, 0)
+        assert torch.equal(got.view(2, nq, d).cpu().double(), one)
+    got = _prompt(get_ops(dev), dev, q, kc, vc, bt, [n, n], [n, n], nq, nkv, d, 0, 0).view(2, n, nq, d)[:, 211:].cpu().double()
+    assert torch.equal(got, one[:, None].expand_as(got))
+
+
+@pytest.mark.parametrize("dev", DEVICES)
+def test_slots_outside_of_the_cache_write_and_read_nothing(dev):
+    """Slots below 0, behind the cache and at the ends of 64 bits, in runs of 16 too."""
+    ops, nq, nkv, d, bs, nb = get_ops(dev), 4, 2, 128, 16, 4
+    slots = torch.cat([torch.arange(-16, 0), torch.arange(nb * bs, nb * bs + 32), torch.arange(-2 ** 63, -2 ** 63 + 32),
+                       2 ** 63 - 32 + torch.arange(32), torch.arange(2 ** 62, 2 ** 62 + 32)])
+    t = len(slots)
+    qkv = _values(torch.Generator().manual_seed(3), t, (nq + 2 * nkv) * d)
+    kc, vc = _random_cache(torch.Generator().manual_seed(4), nb, nkv, bs, d)
+    k, v = kc.to(dev, copy=True), vc.to(dev, copy=True)
+    for n in (t, 100):
+        ops.rope_cache(qkv[:n].to(dev), torch.arange(n, device=dev), slots[:n].to(dev), ref.rope_cos_sin(d, t, 10000.0).to(dev), k, v, nq, nkv, d, 0)
+    assert torch.equal(k.cpu(), kc) and torch.equal(v.cpu(), vc)
+    ko, vo = (torch.ones(t, nkv, d, dtype=torch.bfloat16, device=dev) for _ in "kv")
+    ops.read_cache(ko, vo, k, v, slots.to(dev))
+    assert not ko.any() and not vo.any()
+
+
 @pytest.mark.gpu
 def test_decode_writes_the_f16_copy():
     gen = torch.Generator().manual_seed(2)
@@ -713,6 +788,21 @@ def test_kernel_refusals():
         ops.splitk_rope_cache(q, torch.zeros(1, 2, n - 1, device="cuda"), 1, longs, longs, cs, kc, vc, nq, nkv, d, 0)
     with pytest.raises(RuntimeError):
         ops.splitk_rope_cache(q, torch.zeros(1, 2, n, device="cuda"), 1, longs, longs, cs, kc, vc, nq, nkv, d, 1, q_w=cs[0], k_w=cs[0])
+    # views that do not begin at a multiple of 16 bytes, tables of more than 2^30 tokens
+    off = torch.zeros(kc.numel() + 8, dtype=torch.uint8, device="cuda")[8:].view(kc.shape)
+    wide = torch.zeros(2, nq * d + 2, device="cuda").view(-1)[2:2 + to.numel()].view(to.shape)
+    k256 = torch.zeros(kv4.cache_shape(1, nkv, 256, d), dtype=torch.uint8, device="cuda")
+    long = torch.zeros(2, 2 ** 22 + 1, dtype=torch.int32, device="cuda")
+    for kw in (dict(k=off), dict(v=off), dict(to=wide), dict(k=k256, v=k256, bt=long, window=64)):
+        with pytest.raises(RuntimeError):
+            decode(**kw)
+    with pytest.raises(RuntimeError):
+        ops.rope_cache(q, longs, longs, cs, off, vc, nq, nkv, d, 0)
+    with pytest.raises(RuntimeError):
+        ops.splitk_rope_cache(q, torch.zeros(2 * n + 2, device="cuda")[2:], 1, longs, longs, cs, kc, vc, nq, nkv, d, 0)
+    cu = torch.tensor([0, 2], dtype=torch.int32, device="cuda")
+    with pytest.raises(RuntimeError):
+        ops.prefill_attention(out, q, k256, k256, long, cu, ctx[:1], _tiles([2]).cuda(), nq, nkv, 0.1)
 
 
 # ---------------------------------------------------------------- the engine
@@ -781,6 +871,8 @@ def test_engine_refusals():
         EngineConfig(kv_cache_dtype="fp8", attention_sinks=4)
     with pytest.raises(ValueError):   # heads of 32
         _engine("cpu", PRESETS["tiny-llama"], "float32", kv_cache_dtype="mxfp4")
+    with pytest.raises(ValueError):   # 17 queries per kv head
+        _engine("cpu", _model(heads=17), "float32", kv_cache_dtype="mxfp4")
     with pytest.raises(ValueError):   # a design with caches of its own
         _engine("cpu", PRESETS["tiny-kesirax"], "float32", kv_cache_dtype="mxfp4")
 
