@@ -63,13 +63,44 @@ struct Kv4Tile {
   unsigned char nopage[4];                                          // runs of 16 tokens without a page
 };
 
+// A workgroup's rows and the tiles they see: those of the first `sinks` keys, then those from its first row's window on.
+// Dispatch order: kv-head groups fastest, then the host's tiles, the later rows of a tile first
+struct Kv4Block {
+  int heads, seq, r0, q0, qlen, ctx;  // group of query heads; sequence, first row in it, its first row of all, its rows and length
+  int last, first, nst, nkt;          // last key that some row sees, first tile of the window, tiles of the first keys, tiles in all
+};
+template <int QR>
+HS_DEVICE bool kv4_block(Kv4Block& b, const Kv4Attn& a, const int* __restrict__ cu_q, int seqs, const int* __restrict__ ctx_lens,
+                         int rows, const int* __restrict__ tiles, int L, int groups) {
+  constexpr int SUB = 128 / QR;
+  const int rest = L / groups, t = rest / SUB, sub = SUB - 1 - (rest - t * SUB);
+  b.heads = L - rest * groups;
+  b.seq = tiles[2 * t];
+  b.r0 = tiles[2 * t + 1] + sub * QR;
+  if (b.seq < 0 || b.seq >= seqs) return false;
+  b.q0 = cu_q[b.seq];
+  b.qlen = cu_q[b.seq + 1] - b.q0;
+  if (b.r0 < 0 || b.r0 >= b.qlen || b.q0 < 0 || b.q0 + b.qlen > rows) return false;
+  b.ctx = ctx_lens[b.seq];
+  b.last = min(b.ctx - b.qlen + min(b.r0 + QR - 1, b.qlen - 1), a.bt_width * a.cache.block_size - 1);
+  const int lo = a.window > 0 ? max(0, b.ctx - b.qlen + b.r0 - a.window + 1) : 0;
+  b.first = lo / kKv4Tile;
+  b.nst = min((min(a.sinks, lo) + kKv4Tile - 1) / kKv4Tile, b.first);
+  b.nkt = b.last < 0 ? 0 : max(0, b.nst + b.last / kKv4Tile + 1 - b.first);
+  return true;
+}
+
+// Few rows over a long context: their tiles are cut into up to `splits` runs, a workgroup each, and merged by a second kernel.
+constexpr int kKv4LeastRun = 8;
+HS_HOST_DEVICE int kv4_tile_run(int nkt, int splits) { return max((nkt + splits - 1) / splits, kKv4LeastRun); }
+
 // HG: query heads a workgroup; NWV: its waves; UN: tiles a barrier
 template <int D, int HG, int NWV, int UN>
 __global__ __launch_bounds__(64 * NWV) __attribute__((amdgpu_waves_per_eu(2, 8))) void kv4_prefill_kernel(
     Kv4Attn a, const int* __restrict__ cu_q, int seqs, const int* __restrict__ ctx_lens, int rows,
-    const int* __restrict__ tiles) {
+    const int* __restrict__ tiles, float* __restrict__ work) {
   constexpr int NG = D / 32, KS = (D + 63) / 64;   // scale groups; steps of the first product
-  constexpr int RB = NWV / HG, QR = 32 * RB, SUB = 128 / QR;
+  constexpr int QR = 32 * NWV / HG;
   constexpr int NT = 64 * NWV;
   constexpr int KLD = Kv4Tile<D>::KLD, VLD = Kv4Tile<D>::VLD;
   constexpr int NP = 512 / NT;  // runs of a tile that two waves take
@@ -77,32 +108,29 @@ __global__ __launch_bounds__(64 * NWV) __attribute__((amdgpu_waves_per_eu(2, 8))
   Kv4Tile<D>* buf = reinterpret_cast<Kv4Tile<D>*>(smem);
   __shared__ int nans;  // a value's scale byte of 255 has come by
 
-  // dispatch order: kv-head groups fastest, then the host's tiles, the later rows of a tile first
-  const int L = blockIdx.x + gridDim.x * blockIdx.y, gy = gridDim.y;
-  const int gyi = L % gy, rest = L / gy;
-  const int t = rest / SUB, sub = SUB - 1 - (rest - t * SUB);
-  const int seq = tiles[2 * t], r0 = tiles[2 * t + 1] + sub * QR;
-  if (seq < 0 || seq >= seqs) return;
-  const int q0 = cu_q[seq], qlen = cu_q[seq + 1] - q0;
-  if (r0 < 0 || r0 >= qlen || q0 < 0 || q0 + qlen > rows) return;  // the whole workgroup, before any barrier
+  const int L = blockIdx.x + gridDim.x * blockIdx.y, splits = gridDim.z;
+  Kv4Block blk;
+  if (!kv4_block<QR>(blk, a, cu_q, seqs, ctx_lens, rows, tiles, L, gridDim.y)) return;  // the whole workgroup, before any barrier
+  const int r0 = blk.r0, q0 = blk.q0, qlen = blk.qlen, ctx = blk.ctx, last = blk.last, first = blk.first, nst = blk.nst;
+  const int run = splits > 1 ? kv4_tile_run(blk.nkt, splits) : INT32_MAX / 2;
+  const int v0 = splits > 1 ? run * blockIdx.z : 0, nkt = min(run, blk.nkt - v0);  // this workgroup's tiles, counted from the first of them
+  if (v0 > 0 && nkt <= 0) return;
   const int nkv = a.cache.nkv, bs = a.cache.block_size, G = a.nq / nkv;
-  const int ctx = ctx_lens[seq], cap = a.bt_width * bs;
-  const int kh = gyi / (G / HG);
+  const int cap = a.bt_width * bs;
+  const int kh = blk.heads / (G / HG);
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int h = gyi * HG + wave % HG;
+  const int h = blk.heads * HG + wave % HG;
   const int qi = lane & 31, half = lane >> 5;
   const int wrow0 = r0 + wave / HG * 32;
   const int row = min(wrow0 + qi, qlen - 1);
   const int pos = ctx - qlen + row;                                    // this lane's row
   const int wmin = ctx - qlen + wrow0, wmax = ctx - qlen + min(wrow0 + 31, qlen - 1);  // the wave's
   const int window = a.window, sinks = a.sinks;
-  // tiles of the workgroup: those of the first `sinks` keys, then from its first row's window on
-  const int last = min(ctx - qlen + min(r0 + QR - 1, qlen - 1), cap - 1);  // the last key that some row sees
-  const int lo = window > 0 ? max(0, ctx - qlen + r0 - window + 1) : 0;
-  const int first = lo / kKv4Tile, nst = min((min(sinks, lo) + kKv4Tile - 1) / kKv4Tile, first);
-  const int nkt = last < 0 ? 0 : max(0, nst + last / kKv4Tile + 1 - first);
-  auto tile_key = [&](int v) { return (v < nst ? v : v - nst + first) * kKv4Tile; };
-  const int* bt = a.block_tables + (long)seq * a.bt_stride;
+  auto tile_key = [&](int i) {
+    const int v = i + v0;
+    return (v < nst ? v : v - nst + first) * kKv4Tile;
+  };
+  const int* bt = a.block_tables + (long)blk.seq * a.bt_stride;
   const int bsh = __builtin_ctz(bs), bmask = bs - 1;
 
   // ---- q of this lane's row, on its way first: dims 64 s + 16 half .. and 64 s + 32 + 16 half .. of step s
@@ -441,10 +469,23 @@ __global__ __launch_bounds__(64 * NWV) __attribute__((amdgpu_waves_per_eu(2, 8))
     }
     if (live) values(nkt - 1, buf[(nkt - 1) & 1]);
   }
+  l_run = kv4_sum32(l_run);
+  if (run < blk.nkt) {  // a part of the rows' keys: sums and maxima as they are, a lane's 16 bytes beside its neighbours'
+    if (wrow0 >= qlen) return;
+    const long part = ((long)L * splits + blockIdx.z) * NWV + wave;
+    f32x4* dst = reinterpret_cast<f32x4*>(work + part * 32 * D) + lane;
+#pragma unroll
+    for (int nb = 0; nb < NG; ++nb)
+#pragma unroll
+      for (int g = 0; g < 4; ++g)
+        dst[(4 * nb + g) * 64] = f32x4{o[nb][4 * g], o[nb][4 * g + 1], o[nb][4 * g + 2], o[nb][4 * g + 3]};
+    float* ml = work + (long)gridDim.x * gridDim.y * splits * NWV * 32 * D + part * 64;
+    if (half == 0) *reinterpret_cast<float2*>(ml + 2 * qi) = float2{m_run, l_run};
+    return;
+  }
   // ---- rows through LDS, so that a row's dims leave together
   __syncthreads();
   if (wrow0 >= qlen) return;
-  l_run = kv4_sum32(l_run);
   const float inv = l_run == 0.f ? 0.f : 1.f / l_run;  // a row that sees nothing: zeros
   constexpr int OLD = D + 8;
   static_assert(NWV * 32 * OLD * 2 <= 2 * UN * sizeof(Kv4Tile<D>), "the waves' rows fit the tiles' LDS");
@@ -469,11 +510,70 @@ __global__ __launch_bounds__(64 * NWV) __attribute__((amdgpu_waves_per_eu(2, 8))
   }
 }
 
+// Merges the parts of 32 rows of a head: a wave each, and each for 32 of the dims.
+template <int D, int HG, int NWV>
+__global__ __launch_bounds__(64) void kv4_prefill_merge_kernel(Kv4Attn a, const int* __restrict__ cu_q, int seqs,
+                                                               const int* __restrict__ ctx_lens, int rows,
+                                                               const int* __restrict__ tiles, const float* __restrict__ work, int splits) {
+  constexpr int QR = 32 * NWV / HG;
+  const int L = blockIdx.x / NWV, wave = blockIdx.x % NWV, nb = blockIdx.y;
+  Kv4Block blk;
+  if (!kv4_block<QR>(blk, a, cu_q, seqs, ctx_lens, rows, tiles, L, a.nq / HG)) return;
+  const int run = kv4_tile_run(blk.nkt, splits), parts = (blk.nkt + run - 1) / run;
+  const int lane = threadIdx.x, qi = lane & 31, half = lane >> 5, row = blk.r0 + wave / HG * 32 + qi;
+  if (parts <= 1 || blk.r0 + wave / HG * 32 >= blk.qlen) return;
+  const long part0 = (long)L * splits * NWV + wave;
+  const float* ml = work + (long)gridDim.x * splits * 32 * D + part0 * 64 + 2 * qi;
+  const f32x4* src = reinterpret_cast<const f32x4*>(work + part0 * 32 * D) + nb * 256 + lane;
+  float M = kKv4Least;
+#pragma unroll 4
+  for (int p = 0; p < parts; ++p) M = fmaxf(M, ml[(long)p * NWV * 64]);
+  float l = 0.f;
+  f32x4 o[4];
+#pragma unroll
+  for (int g = 0; g < 4; ++g) o[g] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll 4
+  for (int p = 0; p < parts; ++p) {
+    const float2 x = *reinterpret_cast<const float2*>(ml + (long)p * NWV * 64);
+    const float w = __builtin_amdgcn_exp2f(x.x - M);
+    l += w * x.y;
+#pragma unroll
+    for (int g = 0; g < 4; ++g) o[g] += w * src[(long)p * NWV * 8 * D + 64 * g];
+  }
+  const float inv = l == 0.f ? 0.f : 1.f / l;
+  if (row >= blk.qlen) return;
+  unsigned short* op = static_cast<unsigned short*>(a.out) + (long)(blk.q0 + row) * a.out_stride +
+                       (long)(blk.heads * HG + wave % HG) * D + 32 * nb + 4 * half;
+#pragma unroll
+  for (int g = 0; g < 4; ++g) {
+    u16x4 y;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) y[j] = f32_to_bf16(o[g][j] * inv);
+    *reinterpret_cast<u16x4*>(op + 8 * g) = y;
+  }
+}
+
+// query heads a workgroup: as many as divide a kv head's, up to 8 waves
+static int kv4_prefill_heads(const Kv4Attn& a) {
+  const int G = a.nq / a.cache.nkv;
+  return G % 8 == 0 ? 8 : G % 4 == 0 ? 4 : G % 2 == 0 ? 2 : 1;
+}
+
+int kv4_prefill_splits(const Kv4Attn& a, int ntiles, long* floats) {
+  const int HG = kv4_prefill_heads(a), NWV = HG == 1 ? 4 : 8, QR = 32 * NWV / HG;
+  const long wgs = (long)ntiles * (128 / QR) * (a.nq / HG), slots = HG == 1 ? 512 : 256;  // what the chip holds at once
+  const long cap = (long)a.bt_width * a.cache.block_size;
+  const long seen = a.window > 0 ? min(cap, (long)a.window + a.sinks + QR + 2 * kKv4Tile) : cap;  // at most, by a workgroup
+  const long splits = wgs <= 0 ? 1 : max(1l, min(slots / wgs, seen / kKv4Tile / kKv4LeastRun));
+  *floats = splits > 1 ? wgs * splits * NWV * 32 * (a.cache.D + 2) : 0;
+  return (int)splits;
+}
+
 template <int D, int HG, int NWV>
 static void kv4_prefill(const Kv4Attn& a, const int* cu_q, int seqs, const int* ctx, int rows, const int* tiles, int ntiles,
-                        hipStream_t s) {
-  constexpr int SUB = 128 / (32 * (NWV / HG));
-  constexpr int UN = NWV == 8 ? 2 : 1;  // workgroups of 4 waves come two a compute unit
+                        float* work, int splits, hipStream_t s) {
+  constexpr int SUB = 128 / (32 * NWV / HG);
+  constexpr int UN = NWV == 8 ? 2 : 1;
   constexpr int kLds = 2 * UN * sizeof(Kv4Tile<D>);
   if (kLds > 64 * 1024) {  // more than the default limit: asked for once a device
     static std::atomic<unsigned long> asked{0};
@@ -485,26 +585,28 @@ static void kv4_prefill(const Kv4Attn& a, const int* cu_q, int seqs, const int* 
                             hipFuncAttributeMaxDynamicSharedMemorySize, kLds) == hipSuccess)
       asked.fetch_or(bit, std::memory_order_relaxed);
   }
-  kv4_prefill_kernel<D, HG, NWV, UN><<<dim3(ntiles * SUB, a.nq / HG), 64 * NWV, kLds, s>>>(a, cu_q, seqs, ctx, rows, tiles);
+  kv4_prefill_kernel<D, HG, NWV, UN><<<dim3(ntiles * SUB, a.nq / HG, splits), 64 * NWV, kLds, s>>>(a, cu_q, seqs, ctx, rows, tiles, work);
+  if (splits > 1)
+    kv4_prefill_merge_kernel<D, HG, NWV><<<dim3(ntiles * SUB * (a.nq / HG) * NWV, D / 32), 64, 0, s>>>(a, cu_q, seqs, ctx, rows, tiles, work, splits);
 }
 
-// as many query heads a workgroup as divide a kv head's, up to 8 waves
 template <int D>
 static void kv4_prefill_d(const Kv4Attn& a, const int* cu_q, int seqs, const int* ctx, int rows, const int* tiles, int ntiles,
-                          hipStream_t s) {
-  const int G = a.nq / a.cache.nkv;
-  if (G % 8 == 0) kv4_prefill<D, 8, 8>(a, cu_q, seqs, ctx, rows, tiles, ntiles, s);
-  else if (G % 4 == 0) kv4_prefill<D, 4, 8>(a, cu_q, seqs, ctx, rows, tiles, ntiles, s);
-  else if (G % 2 == 0) kv4_prefill<D, 2, 8>(a, cu_q, seqs, ctx, rows, tiles, ntiles, s);
-  else kv4_prefill<D, 1, 4>(a, cu_q, seqs, ctx, rows, tiles, ntiles, s);
+                          float* work, int splits, hipStream_t s) {
+  switch (kv4_prefill_heads(a)) {
+    case 8: return kv4_prefill<D, 8, 8>(a, cu_q, seqs, ctx, rows, tiles, ntiles, work, splits, s);
+    case 4: return kv4_prefill<D, 4, 8>(a, cu_q, seqs, ctx, rows, tiles, ntiles, work, splits, s);
+    case 2: return kv4_prefill<D, 2, 8>(a, cu_q, seqs, ctx, rows, tiles, ntiles, work, splits, s);
+    default: return kv4_prefill<D, 1, 4>(a, cu_q, seqs, ctx, rows, tiles, ntiles, work, splits, s);
+  }
 }
 
 void launch_kv4_prefill(const Kv4Attn& a, const int* cu_q, int seqs, const int* ctx_lens, int rows, const int* tiles,
-                        int ntiles, hipStream_t s) {
+                        int ntiles, float* work, int splits, hipStream_t s) {
   if (ntiles <= 0) return;
-  if (a.cache.D == 128) kv4_prefill_d<128>(a, cu_q, seqs, ctx_lens, rows, tiles, ntiles, s);
-  else if (a.cache.D == 96) kv4_prefill_d<96>(a, cu_q, seqs, ctx_lens, rows, tiles, ntiles, s);
-  else kv4_prefill_d<64>(a, cu_q, seqs, ctx_lens, rows, tiles, ntiles, s);
+  if (a.cache.D == 128) kv4_prefill_d<128>(a, cu_q, seqs, ctx_lens, rows, tiles, ntiles, work, splits, s);
+  else if (a.cache.D == 96) kv4_prefill_d<96>(a, cu_q, seqs, ctx_lens, rows, tiles, ntiles, work, splits, s);
+  else kv4_prefill_d<64>(a, cu_q, seqs, ctx_lens, rows, tiles, ntiles, work, splits, s);
 }
 
 }  // namespace hipserve

@@ -396,7 +396,12 @@ void prefill_attention_mx4(at::Tensor& out, const at::Tensor& q, const at::Tenso
   const int* ctx = kv4_ints(ctx_lens, k_cache, seqs, "prefill_attention", "context lengths");
   const int* tl = kv4_ints(tiles, k_cache, 0, "prefill_attention", "tiles");
   c10::hip::HIPGuardMasqueradingAsCUDA g(k_cache.device());
-  hipserve::launch_kv4_prefill(a, cu, (int)seqs, ctx, (int)std::min(q.size(0), out.size(0)), tl, (int)tiles.size(0), cur_stream());
+  long floats = 0;  // parts of rows that are split over their keys
+  const int splits = hipserve::kv4_prefill_splits(a, (int)tiles.size(0), &floats);
+  at::Tensor work;
+  if (floats > 0) work = at::empty({floats}, q.options().dtype(at::kFloat));
+  hipserve::launch_kv4_prefill(a, cu, (int)seqs, ctx, (int)std::min(q.size(0), out.size(0)), tl, (int)tiles.size(0),
+                               floats > 0 ? work.data_ptr<float>() : nullptr, splits, cur_stream());
 }
 
 // Per-head RMSNorm of q and k inside the merged qkv rows, in place (Qwen3 / Gemma-3).

@@ -405,6 +405,58 @@ def test_prompt(dev, nq, nkv, d, bs, window, sinks, rows, ctx):
     assert (out[sum(rows):] == 3).all() and (out[:, nq * d:] == 3).all()
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("nq,nkv,d,bs", [(32, 8, 128, 16), (16, 1, 128, 64), (7, 7, 96, 16), (14, 7, 64, 32), (28, 4, 96, 256)])
+@pytest.mark.parametrize("window,sinks", [(0, 0), (2000, 70), (700, 0)])
+@pytest.mark.parametrize("rows,ctx", [([1], [4100]), ([3, 37, 129, 20], [4097, 2500, 700, 20]), ([64, 8, 2], [512, 513, 1100])])
+def test_few_rows_over_long_contexts(nq, nkv, d, bs, window, sinks, rows, ctx):
+    """Rows whose keys are split over workgroups, beside others that are not; a NaN value and a page that is none in one part alone."""
+    gen = torch.Generator().manual_seed(nq + len(rows))
+    nb, bt = _tables(gen, ctx, bs)
+    kc, vc = _random_cache(gen, nb, nkv, bs, d)
+    n = ctx[0]
+    bt[0, n // 4 // bs] = -1
+    tok = n - 40
+    vc.view(nb, nkv, -1)[int(bt[0, tok // bs]), nkv - 1, bs * d // 2 + bs + tok % bs] = 255
+    q = _queries(gen, sum(rows) + 1, nq, nkv, d)
+    want, size = _oracle(q, kc, vc, bt, rows, ctx, nq, nkv, 1 / math.sqrt(d), window, sinks)
+    assert want.isnan().any()
+    out = torch.full((sum(rows) + 1, nq * d), 3.0, device="cuda", dtype=torch.bfloat16)
+    _prompt(get_ops("cuda"), "cuda", q, kc, vc, bt, rows, ctx, nq, nkv, d, window, sinks, out=out)
+    _check(out[:-1], want, size)
+    assert (out[-1] == 3).all()
+
+
+@pytest.mark.gpu
+def test_split_rows_replay():
+    """The workspace of a captured call is the graph's own: replays beside eager calls of other sizes give the eager result."""
+    gen = torch.Generator().manual_seed(8)
+    nq, nkv, d, bs, rows, ctx = 32, 8, 128, 16, [17, 2], [3000, 1500]
+    nb, bt = _tables(gen, ctx, bs)
+    kc, vc = (c.cuda() for c in _random_cache(gen, nb, nkv, bs, d))
+    q = _queries(gen, 19, nq, nkv, d).cuda()
+    args = (bt.cuda(), torch.tensor([0, 17, 19], dtype=torch.int32).cuda(), torch.tensor(ctx, dtype=torch.int32).cuda(), _tiles(rows).cuda())
+    ops, outs = get_ops("cuda"), [torch.empty(19, nq * d, dtype=torch.bfloat16, device="cuda") for _ in range(3)]
+    step = lambda i: ops.prefill_attention(outs[i], q, kc, vc, *args, nq, nkv, 0.1)  # noqa: E731
+    step(0)
+    graphs = []
+    for i in (1, 2):
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            step(i)
+        graphs.append(g)
+    for _ in range(3):
+        q.copy_(torch.randn_like(q))
+        for o in outs:
+            o.fill_(7.0)
+        step(0)
+        for g in graphs:
+            g.replay()
+        torch.empty(1 << 22, device="cuda").fill_(9.0)
+        torch.cuda.synchronize()
+        assert torch.equal(outs[0], outs[1]) and torch.equal(outs[0], outs[2])
+
+
 @pytest.mark.parametrize("dev", DEVICES)
 @pytest.mark.parametrize("d", [64, 96, 128])
 @pytest.mark.parametrize("window,sinks", [(0, 0), (40, 4)])
