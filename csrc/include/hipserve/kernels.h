@@ -89,7 +89,7 @@ struct Kv4Attn {
 void launch_kv4_decode(const Kv4Attn& a, const int* context_lens, float* tmp_out, float* tmp_ml, int B, int part_size,
                        int max_parts, void* out16, hipStream_t s);
 // into how many runs of keys a call's rows are split at most, and the fp32 workspace that takes (0: none)
-int kv4_prefill_splits(const Kv4Attn& a, int ntiles, long* floats);
+int kv4_prefill_splits(const Kv4Attn& a, int seqs, int rows, int ntiles, long* floats);
 void launch_kv4_prefill(const Kv4Attn& a, const int* cu_q, int seqs, const int* ctx_lens, int rows, const int* tiles,
                         int ntiles, float* work, int splits, hipStream_t s);
 

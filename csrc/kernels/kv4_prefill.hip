@@ -64,17 +64,13 @@ struct Kv4Tile {
 };
 
 // A workgroup's rows and the tiles they see: those of the first `sinks` keys, then those from its first row's window on.
-// Dispatch order: kv-head groups fastest, then the host's tiles, the later rows of a tile first
 struct Kv4Block {
-  int heads, seq, r0, q0, qlen, ctx;  // group of query heads; sequence, first row in it, its first row of all, its rows and length
-  int last, first, nst, nkt;          // last key that some row sees, first tile of the window, tiles of the first keys, tiles in all
+  int seq, r0, q0, qlen, ctx;  // sequence, first row in it, its first row of all, its rows and length
+  int last, first, nst, nkt;    // last key that some row sees, first tile of the window, tiles of the first keys, tiles in all
 };
 template <int QR>
 HS_DEVICE bool kv4_block(Kv4Block& b, const Kv4Attn& a, const int* __restrict__ cu_q, int seqs, const int* __restrict__ ctx_lens,
-                         int rows, const int* __restrict__ tiles, int L, int groups) {
-  constexpr int SUB = 128 / QR;
-  const int rest = L / groups, t = rest / SUB, sub = SUB - 1 - (rest - t * SUB);
-  b.heads = L - rest * groups;
+                         int rows, const int* __restrict__ tiles, int t, int sub) {
   b.seq = tiles[2 * t];
   b.r0 = tiles[2 * t + 1] + sub * QR;
   if (b.seq < 0 || b.seq >= seqs) return false;
@@ -90,7 +86,10 @@ HS_DEVICE bool kv4_block(Kv4Block& b, const Kv4Attn& a, const int* __restrict__ 
   return true;
 }
 
-// Few rows over a long context: their tiles are cut into up to `splits` runs, a workgroup each, and merged by a second kernel.
+// Few rows over a long context: their tiles are cut into up to `splits` runs, a workgroup each, and merged by a second kernel: 128 rows at
+// 8192 keys 230 -> 49 us, one row 171 -> 27. A part costs what some 7 tiles do (its sums are 128 KB a workgroup, written and read), so runs of
+// at least 8: with 4 a row of 8192 keys takes 38 us instead of 27, 500 rows of 500 keys 26 instead of 23, and only 64 rows of 1024 less, 23
+// instead of 27.
 constexpr int kKv4LeastRun = 8;
 HS_HOST_DEVICE int kv4_tile_run(int nkt, int splits) { return max((nkt + splits - 1) / splits, kKv4LeastRun); }
 
@@ -98,9 +97,9 @@ HS_HOST_DEVICE int kv4_tile_run(int nkt, int splits) { return max((nkt + splits 
 template <int D, int HG, int NWV, int UN>
 __global__ __launch_bounds__(64 * NWV) __attribute__((amdgpu_waves_per_eu(2, 8))) void kv4_prefill_kernel(
     Kv4Attn a, const int* __restrict__ cu_q, int seqs, const int* __restrict__ ctx_lens, int rows,
-    const int* __restrict__ tiles, float* __restrict__ work) {
+    const int* __restrict__ tiles, bool apart, float* __restrict__ work) {
   constexpr int NG = D / 32, KS = (D + 63) / 64;   // scale groups; steps of the first product
-  constexpr int QR = 32 * NWV / HG;
+  constexpr int QR = 32 * NWV / HG, SUB = 128 / QR;
   constexpr int NT = 64 * NWV;
   constexpr int KLD = Kv4Tile<D>::KLD, VLD = Kv4Tile<D>::VLD;
   constexpr int NP = 512 / NT;  // runs of a tile that two waves take
@@ -108,18 +107,25 @@ __global__ __launch_bounds__(64 * NWV) __attribute__((amdgpu_waves_per_eu(2, 8))
   Kv4Tile<D>* buf = reinterpret_cast<Kv4Tile<D>*>(smem);
   __shared__ int nans;  // a value's scale byte of 255 has come by
 
-  const int L = blockIdx.x + gridDim.x * blockIdx.y, splits = gridDim.z;
+  // Dispatch order: kv-head groups fastest, then the host's tiles, the later rows of a tile first. Workgroups go round the chip's XCDs and
+  // their shader engines in turn, so those of a tile that have no rows (short sequences) must not all come at the same place of that round:
+  // from one tile to the next the order within a tile turns. Where they are many (`apart`), a tile's workgroups come a whole
+  // round of tiles apart, those without rows together: 32 sequences of 20 rows at 4000 keys 182 -> 97 us; one sequence of 4096 rows,
+  // 150 us, would take 158.
+  const int heads = blockIdx.x, t = apart ? blockIdx.y : blockIdx.z;
+  const int sub = (SUB - 1 - (apart ? blockIdx.z : blockIdx.y - blockIdx.z * SUB / 4)) & (SUB - 1);
+  const int splits = apart ? gridDim.z / SUB : 1, split = apart ? blockIdx.z / SUB : 0;
   Kv4Block blk;
-  if (!kv4_block<QR>(blk, a, cu_q, seqs, ctx_lens, rows, tiles, L, gridDim.y)) return;  // the whole workgroup, before any barrier
+  if (!kv4_block<QR>(blk, a, cu_q, seqs, ctx_lens, rows, tiles, t, sub)) return;  // the whole workgroup, before any barrier
   const int r0 = blk.r0, q0 = blk.q0, qlen = blk.qlen, ctx = blk.ctx, last = blk.last, first = blk.first, nst = blk.nst;
   const int run = splits > 1 ? kv4_tile_run(blk.nkt, splits) : INT32_MAX / 2;
-  const int v0 = splits > 1 ? run * blockIdx.z : 0, nkt = min(run, blk.nkt - v0);  // this workgroup's tiles, counted from the first of them
+  const int v0 = splits > 1 ? run * split : 0, nkt = min(run, blk.nkt - v0);  // this workgroup's tiles, counted from the first of them
   if (v0 > 0 && nkt <= 0) return;
   const int nkv = a.cache.nkv, bs = a.cache.block_size, G = a.nq / nkv;
   const int cap = a.bt_width * bs;
-  const int kh = blk.heads / (G / HG);
+  const int kh = heads / (G / HG);
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int h = blk.heads * HG + wave % HG;
+  const int h = heads * HG + wave % HG;
   const int qi = lane & 31, half = lane >> 5;
   const int wrow0 = r0 + wave / HG * 32;
   const int row = min(wrow0 + qi, qlen - 1);
@@ -472,14 +478,15 @@ __global__ __launch_bounds__(64 * NWV) __attribute__((amdgpu_waves_per_eu(2, 8))
   l_run = kv4_sum32(l_run);
   if (run < blk.nkt) {  // a part of the rows' keys: sums and maxima as they are, a lane's 16 bytes beside its neighbours'
     if (wrow0 >= qlen) return;
-    const long part = ((long)L * splits + blockIdx.z) * NWV + wave;
+    const long part = (((long)(t * SUB + sub) * gridDim.x + heads) * splits + split) * NWV + wave;
     f32x4* dst = reinterpret_cast<f32x4*>(work + part * 32 * D) + lane;
+    if (wrow0 + qi >= qlen) return;
 #pragma unroll
     for (int nb = 0; nb < NG; ++nb)
 #pragma unroll
       for (int g = 0; g < 4; ++g)
         dst[(4 * nb + g) * 64] = f32x4{o[nb][4 * g], o[nb][4 * g + 1], o[nb][4 * g + 2], o[nb][4 * g + 3]};
-    float* ml = work + (long)gridDim.x * gridDim.y * splits * NWV * 32 * D + part * 64;
+    float* ml = work + (long)gridDim.x * gridDim.y * gridDim.z * NWV * 32 * D + part * 64;
     if (half == 0) *reinterpret_cast<float2*>(ml + 2 * qi) = float2{m_run, l_run};
     return;
   }
@@ -510,47 +517,45 @@ __global__ __launch_bounds__(64 * NWV) __attribute__((amdgpu_waves_per_eu(2, 8))
   }
 }
 
-// Merges the parts of 32 rows of a head: a wave each, and each for 32 of the dims.
+// Merges the parts of 32 rows of a head: a wave each, and each for 8 of the dims.
 template <int D, int HG, int NWV>
 __global__ __launch_bounds__(64) void kv4_prefill_merge_kernel(Kv4Attn a, const int* __restrict__ cu_q, int seqs,
                                                                const int* __restrict__ ctx_lens, int rows,
                                                                const int* __restrict__ tiles, const float* __restrict__ work, int splits) {
-  constexpr int QR = 32 * NWV / HG;
-  const int L = blockIdx.x / NWV, wave = blockIdx.x % NWV, nb = blockIdx.y;
+  constexpr int QR = 32 * NWV / HG, SUB = 128 / QR;
+  const int heads = blockIdx.x / NWV, wave = blockIdx.x % NWV, t = blockIdx.y / SUB, sub = blockIdx.y % SUB;
   Kv4Block blk;
-  if (!kv4_block<QR>(blk, a, cu_q, seqs, ctx_lens, rows, tiles, L, a.nq / HG)) return;
+  if (!kv4_block<QR>(blk, a, cu_q, seqs, ctx_lens, rows, tiles, t, sub)) return;
   const int run = kv4_tile_run(blk.nkt, splits), parts = (blk.nkt + run - 1) / run;
   const int lane = threadIdx.x, qi = lane & 31, half = lane >> 5, row = blk.r0 + wave / HG * 32 + qi;
-  if (parts <= 1 || blk.r0 + wave / HG * 32 >= blk.qlen) return;
-  const long part0 = (long)L * splits * NWV + wave;
-  const float* ml = work + (long)gridDim.x * splits * 32 * D + part0 * 64 + 2 * qi;
-  const f32x4* src = reinterpret_cast<const f32x4*>(work + part0 * 32 * D) + nb * 256 + lane;
+  if (parts <= 1 || row >= blk.qlen) return;
+  const long part0 = ((long)blockIdx.y * (gridDim.x / NWV) + heads) * splits * NWV + wave;
+  const float* ml = work + (long)gridDim.x * gridDim.y * splits * 32 * D + part0 * 64 + 2 * qi;
+  const f32x4* src = reinterpret_cast<const f32x4*>(work + part0 * 32 * D) + blockIdx.z * 64 + lane;
   float M = kKv4Least;
-#pragma unroll 4
-  for (int p = 0; p < parts; ++p) M = fmaxf(M, ml[(long)p * NWV * 64]);
+  for (int p0 = 0; p0 < parts; p0 += 8)
+#pragma unroll
+    for (int u = 0; u < 8; ++u) M = fmaxf(M, ml[(long)min(p0 + u, parts - 1) * NWV * 64]);
   float l = 0.f;
-  f32x4 o[4];
+  f32x4 o{0.f, 0.f, 0.f, 0.f};
+  for (int p0 = 0; p0 < parts; p0 += 8)
 #pragma unroll
-  for (int g = 0; g < 4; ++g) o[g] = f32x4{0.f, 0.f, 0.f, 0.f};
-#pragma unroll 4
-  for (int p = 0; p < parts; ++p) {
-    const float2 x = *reinterpret_cast<const float2*>(ml + (long)p * NWV * 64);
-    const float w = __builtin_amdgcn_exp2f(x.x - M);
-    l += w * x.y;
-#pragma unroll
-    for (int g = 0; g < 4; ++g) o[g] += w * src[(long)p * NWV * 8 * D + 64 * g];
-  }
+    for (int u = 0; u < 8; ++u) {
+      const int p = min(p0 + u, parts - 1);
+      const float2 x = *reinterpret_cast<const float2*>(ml + (long)p * NWV * 64);
+      const f32x4 y = src[(long)p * NWV * 8 * D];
+      if (p0 + u < parts) {
+        const float w = __builtin_amdgcn_exp2f(x.x - M);
+        l += w * x.y;
+        o += w * y;
+      }
+    }
   const float inv = l == 0.f ? 0.f : 1.f / l;
-  if (row >= blk.qlen) return;
-  unsigned short* op = static_cast<unsigned short*>(a.out) + (long)(blk.q0 + row) * a.out_stride +
-                       (long)(blk.heads * HG + wave % HG) * D + 32 * nb + 4 * half;
+  u16x4 y;
 #pragma unroll
-  for (int g = 0; g < 4; ++g) {
-    u16x4 y;
-#pragma unroll
-    for (int j = 0; j < 4; ++j) y[j] = f32_to_bf16(o[g][j] * inv);
-    *reinterpret_cast<u16x4*>(op + 8 * g) = y;
-  }
+  for (int j = 0; j < 4; ++j) y[j] = f32_to_bf16(o[j] * inv);
+  *reinterpret_cast<u16x4*>(static_cast<unsigned short*>(a.out) + (long)(blk.q0 + row) * a.out_stride +
+                            (long)(heads * HG + wave % HG) * D + 8 * blockIdx.z + 4 * half) = y;
 }
 
 // query heads a workgroup: as many as divide a kv head's, up to 8 waves
@@ -559,12 +564,13 @@ static int kv4_prefill_heads(const Kv4Attn& a) {
   return G % 8 == 0 ? 8 : G % 4 == 0 ? 4 : G % 2 == 0 ? 2 : 1;
 }
 
-int kv4_prefill_splits(const Kv4Attn& a, int ntiles, long* floats) {
+int kv4_prefill_splits(const Kv4Attn& a, int seqs, int rows, int ntiles, long* floats) {
   const int HG = kv4_prefill_heads(a), NWV = HG == 1 ? 4 : 8, QR = 32 * NWV / HG;
   const long wgs = (long)ntiles * (128 / QR) * (a.nq / HG), slots = HG == 1 ? 512 : 256;  // what the chip holds at once
+  const long live = min(wgs, ((long)rows / QR + seqs) * (a.nq / HG));  // that have rows, at most
   const long cap = (long)a.bt_width * a.cache.block_size;
   const long seen = a.window > 0 ? min(cap, (long)a.window + a.sinks + QR + 2 * kKv4Tile) : cap;  // at most, by a workgroup
-  const long splits = wgs <= 0 ? 1 : max(1l, min(slots / wgs, seen / kKv4Tile / kKv4LeastRun));
+  const long splits = live <= 0 || wgs > 2048 ? 1 : max(1l, min(slots / live, seen / kKv4Tile / kKv4LeastRun));
   *floats = splits > 1 ? wgs * splits * NWV * 32 * (a.cache.D + 2) : 0;
   return (int)splits;
 }
@@ -585,9 +591,12 @@ static void kv4_prefill(const Kv4Attn& a, const int* cu_q, int seqs, const int* 
                             hipFuncAttributeMaxDynamicSharedMemorySize, kLds) == hipSuccess)
       asked.fetch_or(bit, std::memory_order_relaxed);
   }
-  kv4_prefill_kernel<D, HG, NWV, UN><<<dim3(ntiles * SUB, a.nq / HG, splits), 64 * NWV, kLds, s>>>(a, cu_q, seqs, ctx, rows, tiles, work);
+  const bool apart = splits > 1 || 4l * rows <= 3l * 128 * ntiles;
+  const int groups = a.nq / HG;
+  kv4_prefill_kernel<D, HG, NWV, UN><<<apart ? dim3(groups, ntiles, SUB * splits) : dim3(groups, SUB, ntiles), 64 * NWV, kLds, s>>>(
+      a, cu_q, seqs, ctx, rows, tiles, apart, work);
   if (splits > 1)
-    kv4_prefill_merge_kernel<D, HG, NWV><<<dim3(ntiles * SUB * (a.nq / HG) * NWV, D / 32), 64, 0, s>>>(a, cu_q, seqs, ctx, rows, tiles, work, splits);
+    kv4_prefill_merge_kernel<D, HG, NWV><<<dim3(groups * NWV, ntiles * SUB, D / 8), 64, 0, s>>>(a, cu_q, seqs, ctx, rows, tiles, work, splits);
 }
 
 template <int D>

@@ -390,17 +390,18 @@ void prefill_attention_mx4(at::Tensor& out, const at::Tensor& q, const at::Tenso
   const hipserve::Kv4Attn a = kv4_attn(out, q, k_cache, v_cache, block_tables, nq, nkv, scale, window, sinks, "prefill_attention");
   const int64_t seqs = cu_q.numel() - 1;
   TORCH_CHECK(seqs >= 0 && block_tables.size(0) >= seqs, "prefill_attention: a block table per sequence");
-  TORCH_CHECK(tiles.dim() == 2 && tiles.size(1) == 2 && tiles.size(0) <= 1 << 20 && tiles.size(0) * nq <= INT32_MAX,
-              "prefill_attention: tiles [tiles, 2], at most 2^20 and 2^31 over the heads");
+  TORCH_CHECK(tiles.dim() == 2 && tiles.size(1) == 2 && tiles.size(0) <= 65535,
+              "prefill_attention: tiles [tiles, 2], at most 65535");
   const int* cu = kv4_ints(cu_q, k_cache, 1, "prefill_attention", "row offsets");
   const int* ctx = kv4_ints(ctx_lens, k_cache, seqs, "prefill_attention", "context lengths");
   const int* tl = kv4_ints(tiles, k_cache, 0, "prefill_attention", "tiles");
   c10::hip::HIPGuardMasqueradingAsCUDA g(k_cache.device());
   long floats = 0;  // parts of rows that are split over their keys
-  const int splits = hipserve::kv4_prefill_splits(a, (int)tiles.size(0), &floats);
+  const int rows = (int)std::min(q.size(0), out.size(0));
+  const int splits = hipserve::kv4_prefill_splits(a, (int)seqs, rows, (int)tiles.size(0), &floats);
   at::Tensor work;
   if (floats > 0) work = at::empty({floats}, q.options().dtype(at::kFloat));
-  hipserve::launch_kv4_prefill(a, cu, (int)seqs, ctx, (int)std::min(q.size(0), out.size(0)), tl, (int)tiles.size(0),
+  hipserve::launch_kv4_prefill(a, cu, (int)seqs, ctx, rows, tl, (int)tiles.size(0),
                                floats > 0 ? work.data_ptr<float>() : nullptr, splits, cur_stream());
 }
 
