@@ -14,7 +14,10 @@
 
 namespace hipserve {
 
-constexpr int kKv4RowsFrom = 128;  // rows from which runs of a page are taken together
+// Rows times kv heads from which runs of a page are taken together, 13 a compute unit: below, a token a workgroup is a shorter chain of loads.
+// Token / runs, us: 32 / 8 heads 64 rows 3.5 / 4.8, 384 rows 5.0 / 5.2, 512 rows 6.1 / 5.4, 8192 rows 40 / 37; 32 / 32 heads 64 rows 4.2 / 4.4,
+// 128 rows 5.6 / 4.6, 8192 rows 119 / 69; 8 / 2 heads 1024 rows 4.2 / 5.1, 2048 rows 5.7 / 5.3.
+constexpr long kKv4RowsFrom = 13 * 256;
 
 struct Kv4In {
   const float* ws;  // split-K partials [S, T, N], or null: the rows of qkv
@@ -293,7 +296,7 @@ static void kv4_write(unsigned short* q, long qkv_stride, const Kv4In& in, const
   auto* kc = static_cast<unsigned char*>(c.k);
   auto* vc = static_cast<unsigned char*>(c.v);
   const long nslots = c.blocks * c.block_size;
-  if (in.ws == nullptr && T >= kKv4RowsFrom) {
+  if (in.ws == nullptr && (long)T * c.nkv >= kKv4RowsFrom) {
 #define HS_KV4_WRITE(mode_)                                                                                              \
   kv4_write_rows_kernel<mode_, D><<<cdiv(T, 16) * c.nkv, 256, 0, s>>>(q, qkv_stride, positions, max_pos, slots, cos_sin, kc, \
                                                                            vc, nslots, T, nq, c.nkv, c.block_size)

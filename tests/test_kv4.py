@@ -190,12 +190,13 @@ def _values(gen, t, n):
 @pytest.mark.parametrize("dev", DEVICES)
 @pytest.mark.parametrize("mode", [0, 1])
 @pytest.mark.parametrize("nq,nkv,d,bs", [(32, 8, 128, 16), (5, 5, 96, 32), (14, 2, 64, 64), (3, 1, 128, 256)])
-@pytest.mark.parametrize("t,order", [(1, "in order"), (37, "anywhere"), (131, "in order"), (260, "aligned")])
+@pytest.mark.parametrize("t,order", [(1, "in order"), (37, "anywhere"), (131, "in order"), (260, "aligned"), (703, "in order"),
+                                     (720, "aligned")])
 def test_write_holds_the_quantised_rows(dev, mode, nq, nkv, d, bs, t, order):
     """The cache's bytes are those of the rows that a bf16 cache holds after the same call, quantised, every other byte is left, and
     the queries are rotated to the same bits; rows in a wider buffer, slots below 0 and behind the cache."""
     gen = torch.Generator().manual_seed(t + d)
-    ops, nb = get_ops(dev), 2 + 600 // bs
+    ops, nb = get_ops(dev), 2 + (t + 600) // bs
     wide = _values(gen, t, (nq + 2 * nkv) * d + 16).to(dev)
     pos = torch.randint(0, 4000, (t,), generator=gen).to(dev)
     slots = {"anywhere": torch.randperm(nb * bs, generator=gen)[:t], "in order": torch.arange(t) + bs + 5,
@@ -234,11 +235,12 @@ def test_write_holds_the_quantised_rows(dev, mode, nq, nkv, d, bs, t, order):
 @pytest.mark.parametrize("dev", DEVICES)
 @pytest.mark.parametrize("mode", [0, 1])
 @pytest.mark.parametrize("nq,nkv,d,bs", [(32, 8, 128, 16), (6, 6, 96, 32), (14, 2, 64, 256), (9, 3, 128, 64)])
-def test_write_and_read_of_ragged_prompts(dev, mode, nq, nkv, d, bs):
-    """A prompt step of many rows: sequences that begin anywhere in the step and in a page, single rows, whole pages, rows of no slot
+@pytest.mark.parametrize("times", [1, 5])
+def test_write_and_read_of_ragged_prompts(dev, mode, nq, nkv, d, bs, times):
+    """Prompt steps of many rows, few and many of them for the writers: sequences that begin anywhere in the step and in a page, single rows, whole pages, rows of no slot
     between them, pages in any order. Written and read rows are the quantised rows of the same call on a bf16 cache."""
     gen = torch.Generator().manual_seed(bs)
-    ops, lens = get_ops(dev), [(0, 70), (5, 6), (0, 1), (3, 100), (16, 48), (0, 131), (9, 10), (0, 16), (250, 300)]
+    ops, lens = get_ops(dev), [(0, 70), (5, 6), (0, 1), (3, 100), (16, 48), (0, 131), (9, 10), (0, 16), (250, 300)] * times
     nb = sum(-(-e // bs) for _, e in lens) + 4
     pages = iter(torch.randperm(nb, generator=gen).tolist())
     slots = []
@@ -248,7 +250,7 @@ def test_write_and_read_of_ragged_prompts(dev, mode, nq, nkv, d, bs):
     last = next(pages)
     slots += [last * bs + o for o in (3, 1, 2, 0, 4)]      # backwards and forwards within a page
     t = len(slots)
-    assert t > 300
+    assert t > 390 * times
     slots = torch.tensor(slots).to(dev)
     n = (nq + 2 * nkv) * d
     x = _values(gen, t, n).to(dev)
