@@ -430,6 +430,46 @@ def test_few_rows_over_long_contexts(nq, nkv, d, bs, window, sinks, rows, ctx):
 
 
 @pytest.mark.gpu
+def test_two_streams_at_once():
+    """Steps of two sequences on streams of their own, at the same time, give what each gives alone."""
+    ops, nq, nkv, d, bs = get_ops("cuda"), 16, 2, 128, 16
+    streams, jobs = [torch.cuda.Stream() for _ in range(2)], []
+    for i in range(2):
+        gen = torch.Generator().manual_seed(30 + i)
+        rows, ctx = [40 + i], [2500 - 700 * i]
+        nb, bt = _tables(gen, ctx, bs)
+        kc, vc = (c.cuda() for c in _random_cache(gen, nb, nkv, bs, d))
+        slots = (bt[0].long()[torch.arange(ctx[0] - rows[0], ctx[0]) // bs] * bs + torch.arange(ctx[0] - rows[0], ctx[0]) % bs).cuda()
+        qkv = _values(gen, rows[0], (nq + 2 * nkv) * d).cuda()
+        parts = -(-bt.shape[1] * bs // 512)
+        jobs.append(dict(rows=rows, qkv=qkv, kc=kc, vc=vc, bt=bt.cuda(), slots=slots, pos=torch.arange(rows[0]).cuda(),
+                         cs=ref.rope_cos_sin(d, 64, 10000.0).cuda(), cu=torch.tensor([0, rows[0]], dtype=torch.int32).cuda(),
+                         ctx=torch.tensor(ctx, dtype=torch.int32).cuda(), tiles=_tiles(rows).cuda(),
+                         to=torch.empty(1, nq, parts, d, device="cuda"), tm=torch.empty(1, nq, parts, 2, device="cuda")))
+
+    def step(j):
+        qkv, kc, vc = j["qkv"].clone(), j["kc"].clone(), j["vc"].clone()
+        out, one = (torch.empty(n, nq * d, dtype=torch.bfloat16, device="cuda") for n in (j["rows"][0], 1))
+        k, v = (torch.empty(j["rows"][0], nkv, d, dtype=torch.bfloat16, device="cuda") for _ in "kv")
+        ops.rope_cache(qkv, j["pos"], j["slots"], j["cs"], kc, vc, nq, nkv, d, 0)
+        ops.read_cache(k, v, kc, vc, j["slots"])
+        ops.prefill_attention(out, qkv, kc, vc, j["bt"], j["cu"], j["ctx"], j["tiles"], nq, nkv, 0.09)
+        ops.paged_decode(one, qkv[-1:], kc, vc, j["bt"], j["ctx"], j["to"], j["tm"], nq, nkv, 512, 0.09)
+        return kc, vc, k, v, out, one
+
+    want = [step(j) for j in jobs]
+    torch.cuda.synchronize()
+    got = []
+    for _ in range(5):
+        for s, j in zip(streams, jobs):
+            with torch.cuda.stream(s):
+                got.append(step(j))
+    torch.cuda.synchronize()
+    for i, g in enumerate(got):
+        assert all(torch.equal(a, b) for a, b in zip(g, want[i % 2]))
+
+
+@pytest.mark.gpu
 def test_split_rows_replay():
     """The workspace of a captured call is the graph's own: replays beside eager calls of other sizes give the eager result."""
     gen = torch.Generator().manual_seed(8)
@@ -914,6 +954,31 @@ def test_engine_matches_dense(window, sinks):
             lg = _dense_logits(m, ids, window, sinks)
             assert lg[t] >= lg.max() - 1e-4
             ids.append(t)
+
+
+def test_engine_reuses_cached_prompts():
+    """A prompt whose beginning is in the cache: the same tokens, with a window and first tokens that stay visible in it."""
+    prompt, sp = list(range(3, 100)), SamplingParams(temperature=0.0, max_tokens=8, ignore_eos=True)
+    want = None
+    for caching in (False, True):
+        eng = _engine("cpu", _model(window=24), "float32", kv_cache_dtype="mxfp4", attention_sinks=4, enable_prefix_caching=caching)
+        got = [eng.generate([p], sp)[0][0] for p in (prompt, prompt, prompt[:70] + [1, 2, 3], prompt)]
+        assert got[0] == got[1] == got[3]
+        want = want or got
+        assert got == want
+
+
+def test_tensor_parallel_engine(tmp_path):
+    """Each of two ranks keeps its kv heads' blocks: the tokens of one rank alone."""
+    from hipserve.weights.safetensors_loader import random_hf_tensors, save_hf_checkpoint
+    from tests import test_tp_cpu as tp
+
+    cfg, ckpt = _model(heads=4, kv_heads=2), str(tmp_path / "kv4")
+    save_hf_checkpoint(ckpt, cfg, random_hf_tensors(cfg, seed=7))
+    eng = LLMEngine(tp._cfg(ckpt, 1, "mxfp4"), tp=TPGroup())
+    assert eng.runner.kv[0][0].dtype == torch.uint8
+    want = [r[0] for r in eng.generate(tp.PROMPTS, SamplingParams(temperature=0.0, max_tokens=8, ignore_eos=True))]
+    assert tp._run_tp(ckpt, 2, "mxfp4") == want
 
 
 def test_engine_refusals():
