@@ -63,30 +63,30 @@ HS_DEVICE unsigned kv4_widen2(unsigned w, float s) {
   return __builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, s, kByte));
 }
 
-// 8 bf16 values over scale (its exponent) as e4m3 numbers hi + lo / 16: the upper four of their eight significant bits, and the rest
+// 8 bf16 values over scale (its exponent) as e4m3 numbers hi + lo / 16: the nearest number to each and what that leaves. The rest is taken
+// from hi as it was converted: where hi is subnormal (below 2^-6) it has fewer than four bits, and lo holds what they lack down to 2^-13.
 HS_DEVICE void kv4_split8(const u16x8 v, float scale, float scale16, u32x2& hi, u32x2& lo) {
   typedef short i16x2 __attribute__((ext_vector_type(2)));
 #pragma unroll
   for (int w = 0; w < 2; ++w) {
-    float h[4], l[4];
+    float x[4];
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const float x = bf16_to_f32(v[4 * w + j]);
-      h[j] = __uint_as_float(__float_as_uint(x) & 0xfff00000u);
-      l[j] = x - h[j];
-    }
+    for (int j = 0; j < 4; ++j) x[j] = bf16_to_f32(v[4 * w + j]);
     i16x2 hp = {0, 0}, lp = {0, 0};
-    hp = __builtin_amdgcn_cvt_scalef32_pk_fp8_f32(hp, h[0], h[1], scale, false);
-    hp = __builtin_amdgcn_cvt_scalef32_pk_fp8_f32(hp, h[2], h[3], scale, true);
-    lp = __builtin_amdgcn_cvt_scalef32_pk_fp8_f32(lp, l[0], l[1], scale16, false);
-    lp = __builtin_amdgcn_cvt_scalef32_pk_fp8_f32(lp, l[2], l[3], scale16, true);
+    hp = __builtin_amdgcn_cvt_scalef32_pk_fp8_f32(hp, x[0], x[1], scale, false);
+    hp = __builtin_amdgcn_cvt_scalef32_pk_fp8_f32(hp, x[2], x[3], scale, true);
     hi[w] = __builtin_bit_cast(unsigned, hp);
+    const auto h0 = __builtin_amdgcn_cvt_scalef32_pk_f32_fp8(hi[w], scale, false);
+    const auto h1 = __builtin_amdgcn_cvt_scalef32_pk_f32_fp8(hi[w], scale, true);
+    lp = __builtin_amdgcn_cvt_scalef32_pk_fp8_f32(lp, x[0] - h0[0], x[1] - h0[1], scale16, false);
+    lp = __builtin_amdgcn_cvt_scalef32_pk_fp8_f32(lp, x[2] - h1[0], x[3] - h1[1], scale16, true);
     lo[w] = __builtin_bit_cast(unsigned, lp);
   }
 }
 
-// Scale bytes of a query's two parts, hi in byte 0, lo in byte 1, from its largest magnitude's bits: that value comes to
-// [128, 256) of e4m3's 448. Of a query that holds a NaN or an infinity both are 255: its scores are NaN.
+// Scale bytes of the two parts of a query's 32 dims (the keys' groups: what is small in q may meet what is large in a key), hi in byte 0,
+// lo in byte 1, from their largest magnitude's bits: that value comes to [128, 256) of e4m3's 448, so values down to 2^-13 of it are exact
+// and smaller ones within 2^-21 of it. Of dims that hold a NaN or an infinity both are 255: the query's scores are NaN.
 HS_DEVICE int kv4_query_scales(unsigned amax_bits) {
   if (amax_bits >= 0x7f80u) return 0xffff;
   const int e = max((int)(amax_bits >> 7), 16);

@@ -6,8 +6,8 @@
 // What bounds it is the cache's bytes (17 D / 32 per token, head and K or V), so nothing is unpacked that need not be:
 //  * scores: K codes go from memory into v_mfma_scale_f32_16x16x128_f8f6f4 as they are, rows = 16 tokens, their scale bytes as its
 //    block scales. The other operand is q in two e4m3 numbers: a bf16 value has 8 significant bits, e4m3 has 4, and what the first
-//    leaves is one e4m3 number again, so q is exact (values below 2^-14 of the row's largest within 2^-21 of it) where one number alone
-//    would lose half of its bits. A power of two per row keeps both in range: the scale byte of that operand.
+//    leaves is one e4m3 number again, so q is exact (values below 2^-13 of the largest of their 32 dims within 2^-21 of it) where one number
+//    alone would lose half of its bits. A power of two per 32 dims, the keys' groups, keeps both in range: the scale bytes of that operand.
 //  * P . V: a byte of V is one token's two dims; v_cvt_scalef32_pk_bf16_fp4 applies the token's scale as it widens, two
 //    v_perm per pair of tokens sort the two dims. Scales ride in the exponent, so a shift makes one of a byte.
 //  * tokens of a 64-key chunk sit so that the lanes that get their scores are the lanes that feed their P: no exchange.
@@ -222,22 +222,17 @@ __global__ __launch_bounds__(64 * kKv4Waves) __attribute__((amdgpu_waves_per_eu(
     pg = next;
   }
   i32x8 qhi[D == 64 ? 2 : 1], qlo[D == 64 ? 2 : 1];
-  int qs;
+  int qs;  // of the dims that this lane's 32 of the product's k are: 32 (grp & 1) .. of 64 dims, 32 grp .. of more
   const float sl = kv4_score_scale(a.scale);
   {
-    unsigned am = 0;
-#pragma unroll
-    for (int h = 0; h < NH; ++h)
-#pragma unroll
-      for (int e = 0; e < 2; ++e)
-        am = max(am, kv4_amax8(raw[h][e]));
-    am = max(am, (unsigned)__shfl_xor((int)am, 16, 64));
-    am = max(am, (unsigned)__shfl_xor((int)am, 32, 64));
-    qs = kv4_query_scales(am);
-    const float down = kv4_scale(qs & 255), down16 = kv4_scale(qs >> 8 & 255);
+    int own[NH];  // of dims 64 h + 32 (grp >> 1) .., which lanes of two grp hold
     u32x4 hi[NH], lo[NH];
 #pragma unroll
-    for (int h = 0; h < NH; ++h)
+    for (int h = 0; h < NH; ++h) {
+      unsigned am = max(kv4_amax8(raw[h][0]), kv4_amax8(raw[h][1]));
+      am = max(am, (unsigned)__shfl_xor((int)am, 16, 64));
+      own[h] = kv4_query_scales(am);
+      const float down = kv4_scale(own[h] & 255), down16 = kv4_scale(own[h] >> 8 & 255);
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
         u32x2 x, y;
@@ -247,6 +242,13 @@ __global__ __launch_bounds__(64 * kKv4Waves) __attribute__((amdgpu_waves_per_eu(
         lo[h][2 * e] = y[0];
         lo[h][2 * e + 1] = y[1];
       }
+    }
+    const int from = col + 32 * (grp & 1);
+    qs = __shfl(own[0], from, 64);
+    if constexpr (NH == 2) {
+      const int second = __shfl(own[1], from, 64);
+      if (grp >= 2) qs = second;
+    }
     const u32x4 z{0, 0, 0, 0};
     if constexpr (D == 64) {
       qhi[0] = kv4_pad(hi[0], z);

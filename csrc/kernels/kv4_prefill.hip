@@ -11,7 +11,7 @@
 //    Each at the other's shape is slower: 8 waves by the second 887 against 840 us (4096 rows at 16384, 32 / 8 heads), 4 waves by
 //    the first 124 against 111 us (8 x 1024 rows, 32 / 32 heads).
 //  * S^T = K . Q^T on v_mfma_scale_f32_32x32x64_f8f6f4: K's codes lie in LDS as they are (a quarter of bf16's LDS reads), their
-//    scale bytes are the product's; q as two e4m3 numbers (see kv4_decode.hip), exact for a bf16 q, at bf16's rate.
+//    scale bytes are the product's; q as two e4m3 numbers (see kv4_decode.hip), the bits of a bf16 q, at bf16's rate.
 //  * V is widened to bf16 on its way into LDS, transposed as it lies in the cache: a thread takes 8 tokens of two dims, v_cvt applies the
 //    scales, v_perm sorts the dims.
 //  * keys sit in K's LDS rows with bits 2 and 3 exchanged: a lane's scores are then 8 neighbouring keys a step of the second product,
@@ -242,23 +242,21 @@ __global__ __launch_bounds__(64 * NWV) __attribute__((amdgpu_waves_per_eu(2, 8))
     ask(UN);
   }
 
-  // ---- q's two parts
+  // ---- q's two parts, a scale per 32 dims (see kv4.h)
   i32x8 qhi[KS], qlo[KS];
-  int qs;
+  int qs[KS];  // of the dims that this lane's 32 of a step's k are: 64 s + 32 half ..
   const float sl = kv4_score_scale(a.scale);
-  {
-    unsigned am = 0;
 #pragma unroll
-    for (int s = 0; s < KS; ++s)
+  for (int s = 0; s < KS; ++s) {
 #pragma unroll
-      for (int e = 0; e < 4; ++e) am = max(am, kv4_amax8(raw[s][e]));
-    am = max(am, (unsigned)__shfl_xor((int)am, 32, 64));
-    qs = kv4_query_scales(am);
-    const float down = kv4_scale(qs & 255), down16 = kv4_scale(qs >> 8 & 255);
+    for (int g = 0; g < 2; ++g) {
+      unsigned am = max(kv4_amax8(raw[s][2 * g]), kv4_amax8(raw[s][2 * g + 1]));
+      am = max(am, (unsigned)__shfl_xor((int)am, 32, 64));
+      const int own = kv4_query_scales(am);
+      if (g == 0 || half) qs[s] = own;
+      const float down = kv4_scale(own & 255), down16 = kv4_scale(own >> 8 & 255);
 #pragma unroll
-    for (int s = 0; s < KS; ++s)
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
+      for (int e = 2 * g; e < 2 * g + 2; ++e) {
         u32x2 hi, lo2;
         kv4_split8(raw[s][e], down, down16, hi, lo2);
         qhi[s][2 * e] = (int)hi[0];
@@ -266,6 +264,7 @@ __global__ __launch_bounds__(64 * NWV) __attribute__((amdgpu_waves_per_eu(2, 8))
         qlo[s][2 * e] = (int)lo2[0];
         qlo[s][2 * e + 1] = (int)lo2[1];
       }
+    }
   }
 
   f32x16 o[NG], st[2];
@@ -302,10 +301,10 @@ __global__ __launch_bounds__(64 * NWV) __attribute__((amdgpu_waves_per_eu(2, 8))
       }
 #pragma unroll
       for (int h2 = 0; h2 < 2; ++h2)
-        st[h2] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(kv4_pad(kf[h2]), qlo[s], st[h2], 4, 0, 0, ks[h2], 1, qs);
+        st[h2] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(kv4_pad(kf[h2]), qlo[s], st[h2], 4, 0, 0, ks[h2], 1, qs[s]);
 #pragma unroll
       for (int h2 = 0; h2 < 2; ++h2)
-        st[h2] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(kv4_pad(kf[h2]), qhi[s], st[h2], 4, 0, 0, ks[h2], 0, qs);
+        st[h2] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(kv4_pad(kf[h2]), qhi[s], st[h2], 4, 0, 0, ks[h2], 0, qs[s]);
     }
   };
   auto softmax = [&](int v, const Kv4Tile<D>& b) __attribute__((always_inline)) {

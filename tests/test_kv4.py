@@ -407,6 +407,67 @@ def test_prompt(dev, nq, nkv, d, bs, window, sinks, rows, ctx):
     assert (out[sum(rows):] == 3).all() and (out[:, nq * d:] == 3).all()
 
 
+@pytest.mark.parametrize("dev", DEVICES)
+@pytest.mark.parametrize("nq,nkv,d,bs", [(32, 8, 128, 16), (7, 7, 96, 16), (28, 4, 64, 32), (16, 1, 96, 64)])
+@pytest.mark.parametrize("powers", [(0, 0, -24, 24), (20, -12, 0, 8), (-24, 0, 16, -8)])
+def test_queries_small_where_keys_are_large(dev, nq, nkv, d, bs, powers):
+    """The query's 32 dims of a key's group 2^power, the key's 2^-power: every group says as much of the score as in the other tests.
+    Within a group the query's magnitudes are within a factor of 2^8, so a sum of two e4m3 numbers has all their bits and the usual bound holds."""
+    gen = torch.Generator().manual_seed(nq + powers[0])
+    ctx = [1, 40, 300, 517]
+    nb, bt = _tables(gen, ctx, bs)
+    kc, vc = _random_cache(gen, nb, nkv, bs, d, spread=1)
+    size = torch.rand(404, nq + 2 * nkv, d, generator=gen) * 2 + 2.0 ** -6
+    q = size * (torch.randint(0, 2, size.shape, generator=gen) * 2 - 1)
+    for g in range(d // 32):
+        q[..., 32 * g:32 * g + 32] *= 2.0 ** powers[g]
+        by_group = kc.view(nb, nkv, -1)[..., bs * d // 2:].view(nb, nkv, d // 32, bs)
+        by_group[:, :, g] -= powers[g] % 256
+    q = q.flatten(1).to(torch.bfloat16)
+    rows = [1, 3, 300, 100]
+    want, size = _oracle(q, kc, vc, bt, rows, ctx, nq, nkv, 1 / math.sqrt(d), 0, 0)
+    _check(_prompt(get_ops(dev), dev, q[:404], kc, vc, bt, rows, ctx, nq, nkv, d, 0, 0), want, size)
+    want, size = _oracle(q[:4], kc, vc, bt, [1] * 4, ctx, nq, nkv, 1 / math.sqrt(d), 0, 0)
+    for part in (64, 1024):
+        _check(_decode(get_ops(dev), dev, q[:4], kc, vc, bt, ctx, nq, nkv, d, bs, part, 0, 0), want, size)
+
+
+@pytest.mark.parametrize("dev", DEVICES)
+@pytest.mark.parametrize("d", [64, 96, 128])
+@pytest.mark.parametrize("dim", [1, 31, 40, 63])
+def test_small_values_of_a_query_beside_a_large_one(dev, d, dim):
+    """All 128 mantissas of 2^-8 .. 2^-20 beside a largest value of 1 (the one that leaves the fewest bits) in the same 32 dims: the first key
+    meets the small value alone, with a score of 1 to 3, the second one nothing.
+
+    Two e4m3 numbers hold a value within 2^-21 of the largest, exactly from 2^-13 of it on; the score is one product. The output is
+    6 / (1 + exp(-score)), of slope 6 / 4 at most."""
+    nq, nkv, bs, low = 16, 1, 16, range(8, 21)
+    kc, vc = (torch.zeros(kv4.cache_shape(len(low), nkv, bs, d), dtype=torch.uint8) for _ in "kv")
+    k, v = kc.view(len(low), -1), vc.view(len(low), -1)
+    k[:, bs * d // 2:], v[:, bs * d // 2:] = 127, 127
+    k[:, dim // 2] = 7 << 4 * (dim % 2)                        # token 0: 6 of a unit that makes the score
+    v[:, :bs * d // 2:bs] = 0x77                               # token 0: 6, token 1: 0
+    scale, up = 1 / math.sqrt(d), [r + 1 for r in low]         # 6 2^-r 2^(r + 1) / sqrt(d): from 1.06 on
+    for i, b in enumerate(up):
+        k[i, bs * d // 2 + dim // 32 * bs] = 127 + b
+    x = torch.tensor([[(1 + m / 128) * 2.0 ** -r for m in range(128)] for r in low], dtype=torch.float64)
+    n = x.numel() // nq
+    q = torch.zeros(n, nq + 2 * nkv, d)
+    q[:, :nq, dim] = x.view(n, nq).float()
+    q[:, :nq, dim // 32 * 32 + 2] = 1.0
+    q = q.flatten(1).to(torch.bfloat16)
+    bt = torch.arange(len(low), dtype=torch.int32).repeat_interleave(128 // nq)[:, None]
+    unit = 6 * torch.exp2(torch.tensor(up, dtype=torch.float64)) * scale
+    want = 6 / (1 + torch.exp(-x * unit[:, None]))
+    lost = torch.where(x < 2.0 ** -13, 2.0 ** -21, 0.0) * unit[:, None]
+    # beside the lost bits: the probability's and the output's rounding, and the 32-bit steps of _check
+    tol = (6 / 4 * lost + (2 ** -8 + 2 ** -11 + 2 ** -8) * want).view(n, nq, 1)
+    for got in (_decode(get_ops(dev), dev, q, kc, vc, bt, [2] * n, nq, nkv, d, bs, 64, 0, 0),
+                _prompt(get_ops(dev), dev, q, kc, vc, bt, [1] * n, [2] * n, nq, nkv, d, 0, 0)):
+        off = (got.float().cpu().double().view(n, nq, d) - want.view(n, nq, 1)).abs()
+        assert (off <= tol).all(), f"off by {(off / tol).max():.3f} of what the query's parts allow"
+
+
 @pytest.mark.gpu
 @pytest.mark.parametrize("nq,nkv,d,bs", [(32, 8, 128, 16), (16, 1, 128, 64), (7, 7, 96, 16), (14, 7, 64, 32), (28, 4, 96, 256)])
 @pytest.mark.parametrize("window,sinks", [(0, 0), (2000, 70), (700, 0)])
