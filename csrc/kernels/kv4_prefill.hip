@@ -80,9 +80,10 @@ HS_DEVICE bool kv4_block(Kv4Block& b, const Kv4Attn& a, const int* __restrict__ 
   b.ctx = ctx_lens[b.seq];
   b.last = min(b.ctx - b.qlen + min(b.r0 + QR - 1, b.qlen - 1), a.bt_width * a.cache.block_size - 1);
   const int lo = a.window > 0 ? max(0, b.ctx - b.qlen + b.r0 - a.window + 1) : 0;
+  const int end = b.last < 0 ? 0 : b.last / kKv4Tile + 1;  // tiles that the table has keys of: a length may go beyond it
   b.first = lo / kKv4Tile;
-  b.nst = min((min(a.sinks, lo) + kKv4Tile - 1) / kKv4Tile, b.first);
-  b.nkt = b.last < 0 ? 0 : max(0, b.nst + b.last / kKv4Tile + 1 - b.first);
+  b.nst = min((min(a.sinks, lo) + kKv4Tile - 1) / kKv4Tile, min(b.first, end));
+  b.nkt = b.nst + max(0, end - b.first);
   return true;
 }
 

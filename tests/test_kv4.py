@@ -679,6 +679,22 @@ def test_a_length_beyond_the_table_ends_with_it(dev):
 
 
 @pytest.mark.parametrize("dev", DEVICES)
+@pytest.mark.parametrize("nq,nkv,d,bs", [(16, 2, 128, 16), (8, 2, 96, 32), (4, 2, 64, 16), (3, 3, 128, 64)])
+@pytest.mark.parametrize("window,sinks", [(100, 4), (100, 0), (1, 70), (100, 1000), (0, 0), (300, 2 ** 31 - 1)])
+@pytest.mark.parametrize("held,rows,ctx", [(512, [3, 70, 260, 5], [700, 560, 640, 512]), (4096, [1, 2], [9000, 4100])])
+def test_prompt_rows_beyond_their_table(dev, nq, nkv, d, bs, window, sinks, held, rows, ctx):
+    """Prompt: positions go on behind the table's keys, so a window may lie wholly behind them; the first tokens are seen all the same."""
+    gen = torch.Generator().manual_seed(sum(ctx) + nq)
+    nb, bt = _tables(gen, [held] * len(ctx), bs)
+    kc, vc = _random_cache(gen, nb, nkv, bs, d)
+    q = _queries(gen, sum(rows), nq, nkv, d)
+    more = torch.cat((bt, torch.full((len(ctx), -(-max(ctx) // bs)), -1, dtype=torch.int32)), 1)   # no pages there
+    want, size = _oracle(q, kc, vc, more, rows, ctx, nq, nkv, 1 / math.sqrt(d), window, sinks)
+    assert bool(want[:rows[0]].any()) == (sinks > 0 or window != 100 and window != 1)
+    _check(_prompt(get_ops(dev), dev, q, kc, vc, bt, rows, ctx, nq, nkv, d, window, sinks), want, size)
+
+
+@pytest.mark.parametrize("dev", DEVICES)
 @pytest.mark.parametrize("d", [64, 96, 128])
 def test_scores_at_the_ends_of_the_range(dev, d):
     """Scores around -2^110 (one product each, so exact): the least negative one takes all, wherever it stands; the others' weights are 0,
