@@ -533,7 +533,7 @@ class EngineConfig:
     # head; 4.25 bits, 3.76x the KV blocks of bf16; ops/kv4.py)
     kv_cache_dtype: str = "auto"
     # sliding-window layers: the first tokens of a sequence that stay visible beside the window
-    # (mxfp4 KV cache; 0 = the window alone, as the model was trained)
+    # (mxfp4 KV cache and a model that has such layers; 0 = the window alone, as the model was trained)
     attention_sinks: int = 0
     host: str = "0.0.0.0"
     port: int = 8080

@@ -122,6 +122,9 @@ class ModelRunner:
             if self.model.nq > 16 * self.model.nkv:
                 raise ValueError(f"{mcfg.name}: the mxfp4 KV cache serves up to 16 queries per kv head, not "
                                  f"{self.model.nq // self.model.nkv}")
+            if ecfg.attention_sinks and not any(mcfg.layer_windows):
+                raise ValueError(f"{mcfg.name}: attention_sinks keeps first tokens visible beside a sliding window, and no layer of this "
+                                 "model has one")
             self.model.kv_dtype = kv4.DTYPE
             self.model.fused_qkv_attention = False
             self.model.attention_sinks = ecfg.attention_sinks

@@ -45,7 +45,8 @@ def build_parser(prog="hipserve") -> argparse.ArgumentParser:
                     help="paged KV cache element: auto (bf16), fp8 (e4m3, per-tensor scale 1: 2x the KV blocks) or mxfp4 (4 bits, a scale per "
                          "32 dims: 3.76x the KV blocks)")
     ap.add_argument("--attention-sinks", type=int, default=0,
-                    help="sliding-window layers over an mxfp4 KV cache: first tokens that stay visible beside the window")
+                    help="sliding-window layers over an mxfp4 KV cache: first tokens that stay visible beside the window "
+                         "(refused for a model without such layers)")
     ap.add_argument("--max-num-seqs", type=int, default=256)
     ap.add_argument("--max-num-batched-tokens", type=int, default=None,
                     help="prefill token budget per step (default 8192; 16384 for GGUF weights)")

@@ -1073,6 +1073,16 @@ def test_engine_refusals():
         _engine("cpu", PRESETS["tiny-kesirax"], "float32", kv_cache_dtype="mxfp4")
 
 
+def test_first_tokens_need_a_windowed_layer():
+    """Without one the flag would change nothing; one windowed layer among others will do."""
+    with pytest.raises(ValueError, match="no layer"):
+        _engine("cpu", _model(), "float32", kv_cache_dtype="mxfp4", attention_sinks=4)
+    with pytest.raises(ValueError, match="no layer"):
+        _engine("cpu", _model().replace(layer_windows=(0, 0)), "float32", kv_cache_dtype="mxfp4", attention_sinks=4)
+    mixed = _model(window=24).replace(layer_windows=(24, 0))
+    assert _engine("cpu", mixed, "float32", kv_cache_dtype="mxfp4", attention_sinks=4).runner.model.attention_sinks == 4
+
+
 def test_command_line():
     from hipserve.server import cli
 
