@@ -75,9 +75,11 @@ HS_DEVICE bool kv4_block(Kv4Block& b, const Kv4Attn& a, const int* __restrict__ 
   b.r0 = tiles[2 * t + 1] + sub * QR;
   if (b.seq < 0 || b.seq >= seqs) return false;
   b.q0 = cu_q[b.seq];
-  b.qlen = cu_q[b.seq + 1] - b.q0;
-  if (b.r0 < 0 || b.r0 >= b.qlen || b.q0 < 0 || b.q0 + b.qlen > rows) return false;
-  b.ctx = ctx_lens[b.seq];
+  const int q1 = cu_q[b.seq + 1];
+  if (b.q0 < 0 || q1 < b.q0 || q1 > rows) return false;  // before their difference, which others may have beyond 32 bits
+  b.qlen = q1 - b.q0;
+  if (b.r0 < 0 || b.r0 >= b.qlen) return false;
+  b.ctx = max(ctx_lens[b.seq], 0);
   b.last = min(b.ctx - b.qlen + min(b.r0 + QR - 1, b.qlen - 1), a.bt_width * a.cache.block_size - 1);
   const int lo = a.window > 0 ? max(0, b.ctx - b.qlen + b.r0 - a.window + 1) : 0;
   const int end = b.last < 0 ? 0 : b.last / kKv4Tile + 1;  // tiles that the table has keys of: a length may go beyond it

@@ -114,7 +114,7 @@ def load(cache, slots, values: bool) -> torch.Tensor:
 def context(k_cache, v_cache, block_table, n: int):
     """(keys, values, page present) of the first n tokens of a sequence: a block id outside of the cache is no page."""
     bs = k_cache.shape[2]
-    j = torch.arange(min(n, block_table.shape[0] * bs), device=k_cache.device)
+    j = torch.arange(max(0, min(n, block_table.shape[0] * bs)), device=k_cache.device)
     page = block_table[j // bs].long()
     ok = (page >= 0) & (page < k_cache.shape[0])
     slots = torch.where(ok, page * bs + j % bs, -1)

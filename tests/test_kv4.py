@@ -695,6 +695,37 @@ def test_prompt_rows_beyond_their_table(dev, nq, nkv, d, bs, window, sinks, held
 
 
 @pytest.mark.parametrize("dev", DEVICES)
+@pytest.mark.parametrize("length", [0, -1, -2 ** 31 + 1, -2 ** 31])
+def test_a_prompt_of_no_length_is_zeros(dev, length):
+    """Rows before position 0 see nothing, however far before."""
+    gen = torch.Generator().manual_seed(24)
+    nq, nkv, d, bs = 8, 2, 128, 16
+    nb, bt = _tables(gen, [64, 64], bs)
+    kc, vc = _random_cache(gen, nb, nkv, bs, d)
+    q = _queries(gen, 10, nq, nkv, d)
+    for window, sinks in ((0, 0), (20, 4)):
+        out = _prompt(get_ops(dev), dev, q, kc, vc, bt, [3, 7], [length, 64], nq, nkv, d, window, sinks)
+        want, size = _oracle(q[3:], kc, vc, bt[1:], [7], [64], nq, nkv, 1 / math.sqrt(d), window, sinks)
+        assert not out[:3].any()
+        _check(out[3:], want, size)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("cu", [[1, -2 ** 31], [2, -2 ** 31 + 1], [0, 2 ** 31 - 1], [-2 ** 31, 5], [-1, 2], [5, 3], [0, 11], [2 ** 31 - 1, -2 ** 31]])
+def test_row_offsets_out_of_range_compute_nothing(cu):
+    """Offsets that go back, or leave the rows, differences beyond 32 bits among them: no row is written."""
+    gen = torch.Generator().manual_seed(25)
+    nq, nkv, d, bs = 8, 2, 128, 16
+    nb, bt = _tables(gen, [64], bs)
+    kc, vc = (c.cuda() for c in _random_cache(gen, nb, nkv, bs, d))
+    q = _queries(gen, 10, nq, nkv, d).cuda()
+    out = torch.full((10, nq * d), 3.0, device="cuda", dtype=torch.bfloat16)
+    ints = lambda *x: torch.tensor(x, device="cuda", dtype=torch.int32)  # noqa: E731
+    get_ops("cuda").prefill_attention(out, q, kc, vc, bt.cuda(), ints(*cu), ints(64), ints(0, 0).view(1, 2), nq, nkv, 0.1)
+    assert (out == 3).all()
+
+
+@pytest.mark.parametrize("dev", DEVICES)
 @pytest.mark.parametrize("d", [64, 96, 128])
 def test_scores_at_the_ends_of_the_range(dev, d):
     """Scores around -2^110 (one product each, so exact): the least negative one takes all, wherever it stands; the others' weights are 0,
