@@ -372,6 +372,9 @@ void paged_decode_mx4(at::Tensor& out, const at::Tensor& q, const at::Tensor& k_
   const int64_t B = q.size(0);
   TORCH_CHECK(out.size(0) >= B && block_tables.size(0) >= B && B < 65536, "paged_decode: rows of out and of the block tables");
   const int* ctx = kv4_ints(context_lens, k_cache, B, "paged_decode", "context lengths");
+  // the kernel cuts all sequences' keys into runs by their number of chunks of 64, which it counts in 32 bits
+  TORCH_CHECK(B * (block_tables.size(1) * a.cache.block_size / 64 + 1) <= INT32_MAX,
+              "paged_decode: block tables of over 2^31 chunks of 64 tokens in all");
   TORCH_CHECK(part_size > 0 && part_size % 64 == 0 && part_size <= 16384, "paged_decode: partitions of a multiple of 64 tokens, at most 16384");
   for (const at::Tensor* t : {&tmp_out, &tmp_ml})
     TORCH_CHECK(t->device() == k_cache.device() && t->scalar_type() == at::kFloat && t->is_contiguous() && t->dim() == 4 &&

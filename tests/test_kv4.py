@@ -1007,6 +1007,18 @@ def test_kernel_refusals():
         ops.prefill_attention(out, q, k256, k256, long, cu, ctx[:1], _tiles([2]).cuda(), nq, nkv, 0.1)
 
 
+@pytest.mark.gpu
+def test_decode_refuses_more_keys_than_it_counts():
+    """Rows that share one long table: 2^24 chunks of 64 tokens each, 2^31 of them together."""
+    nq, nkv, d, rows = 1, 1, 64, 128
+    kc = torch.zeros(kv4.cache_shape(1, nkv, 256, d), dtype=torch.uint8, device="cuda")
+    bt = torch.zeros(1, 2 ** 22, dtype=torch.int32, device="cuda").expand(rows, -1)
+    q = torch.zeros(rows, nq * d, dtype=torch.bfloat16, device="cuda")
+    ctx, to, tm = torch.ones(rows, dtype=torch.int32, device="cuda"), torch.zeros(rows, nq, 1, d, device="cuda"), torch.zeros(rows, nq, 1, 2, device="cuda")
+    with pytest.raises(RuntimeError, match="chunks of 64 tokens in all"):
+        get_ops("cuda").paged_decode(q.clone(), q, kc, kc, bt, ctx, to, tm, nq, nkv, 16384, 0.1)
+
+
 # ---------------------------------------------------------------- the engine
 
 def _model(heads=2, kv_heads=1, dim=64, window=0, layers=2):
