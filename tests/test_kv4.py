@@ -468,6 +468,135 @@ def test_small_values_of_a_query_beside_a_large_one(dev, d, dim):
         assert (off <= tol).all(), f"off by {(off / tol).max():.3f} of what the query's parts allow"
 
 
+def _chunks(n, window, sinks):
+    """Chunks of 64 keys that a decode row of n keys takes: those of the first keys, then the window's."""
+    lo = max(0, n - window) if window else 0
+    return min(-(-min(sinks, lo) // 64), lo // 64) + -(-n // 64) - lo // 64 if n else 0
+
+
+def _run_chunks(ctx, nkv, parts, window, sinks):
+    """Chunks of a decode workgroup's run, a fourth of them a wave's: by what 512 workgroups take, or the workspace's partitions."""
+    count = [_chunks(n, window, sinks) for n in ctx]
+    slots = max(512 - len(ctx) * nkv // 2, 256)
+    return -(-max(sum(count) * nkv // slots + 1, -(-max(count) // parts)) // 4) * 4
+
+
+def _spoil(caches, bt, bs, d, seq, tok, head, group):
+    """A value group's scale byte to that of NaN."""
+    v = caches[1].view(caches[1].shape[0], caches[1].shape[1], -1)
+    v[int(bt[seq, tok // bs]), head, bs * d // 2 + group * bs + tok % bs] = 255
+
+
+LONG = [(32, 8, 128, 16), (16, 1, 128, 64), (7, 7, 96, 16), (28, 4, 64, 32)]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("nq,nkv,d,bs", LONG)
+@pytest.mark.parametrize("window,sinks", [(0, 0), (1100, 70), (900, 0)])
+def test_decode_of_many_chunks_a_wave(nq, nkv, d, bs, window, sinks):
+    """One partition a row: each of the four waves takes up to eight chunks, its two sets of registers in turn; odd ends, and a NaN value and a
+    page that is none in late chunks."""
+    gen = torch.Generator().manual_seed(nq + d)
+    ctx = [1200, 1217, 2000, 770, 0, 1, 1151]
+    nb, bt = _tables(gen, ctx, bs)
+    kc, vc = _random_cache(gen, nb, nkv, bs, d)
+    _spoil((kc, vc), bt, bs, d, 1, 1180, nkv - 1, 1)
+    bt[2, 1900 // bs] = -1
+    q = _queries(gen, len(ctx), nq, nkv, d)
+    assert bt.shape[1] * bs <= 2048 and _chunks(2000, window, sinks) >= 4 * 3
+    want, size = _oracle_rows(q, kc, vc, bt, ctx, nq, nkv, d, window, sinks)
+    assert want[1].isnan().any()
+    _check(_decode(get_ops("cuda"), "cuda", q, kc, vc, bt, ctx, nq, nkv, d, bs, 2048, window, sinks), want, size)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("nq,nkv,d,bs", LONG)
+@pytest.mark.parametrize("window,sinks", [(0, 0), (4300, 70)])
+def test_decode_of_many_chunks_a_run(nq, nkv, d, bs, window, sinks):
+    """Rows in few partitions of many chunks each; a NaN value and pages that are none in the last run and in one between."""
+    gen = torch.Generator().manual_seed(nq + d + 1)
+    ctx = [8200, 4999, 130]
+    nb, bt = _tables(gen, ctx, bs)
+    kc, vc = _random_cache(gen, nb, nkv, bs, d)
+    _spoil((kc, vc), bt, bs, d, 0, 8150, 0, 0)
+    bt[0, 6000 // bs], bt[1, 4900 // bs] = nb, -1
+    q = _queries(gen, len(ctx), nq, nkv, d)
+    parts = -(-bt.shape[1] * bs // 2048)
+    assert _run_chunks(ctx, nkv, parts, window, sinks) >= 4 * 3
+    want, size = _oracle(q, kc, vc, bt, [1] * 3, ctx, nq, nkv, 1 / math.sqrt(d), window, sinks)
+    assert want[0].isnan().any()
+    _check(_decode(get_ops("cuda"), "cuda", q, kc, vc, bt, ctx, nq, nkv, d, bs, 2048, window, sinks), want, size)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("nq,nkv,d,bs,n", [(4, 1, 128, 16, 8300), (16, 1, 96, 32, 10500), (2, 1, 64, 16, 17000)])
+def test_decode_of_more_runs_than_the_merge_takes_at_once(nq, nkv, d, bs, n):
+    """One kv head: a row's runs are as many as 512 workgroups allow, more than the merge's lanes take four each."""
+    gen = torch.Generator().manual_seed(n)
+    ctx = [n, 700]
+    nb, bt = _tables(gen, ctx, bs)
+    kc, vc = _random_cache(gen, nb, nkv, bs, d)
+    q = _queries(gen, 2, nq, nkv, d)
+    runs = -(-_chunks(n, 0, 0) // _run_chunks(ctx, nkv, -(-bt.shape[1] * bs // 64), 0, 0))
+    assert runs > 4 * (256 // (d // 4))
+    want, size = _oracle(q, kc, vc, bt, [1, 1], ctx, nq, nkv, 1 / math.sqrt(d), 0, 0)
+    _check(_decode(get_ops("cuda"), "cuda", q, kc, vc, bt, ctx, nq, nkv, d, bs, 64, 0, 0), want, size)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("nq,nkv,d,bs", [(4, 1, 128, 16), (4, 2, 64, 32), (3, 3, 96, 16)])
+@pytest.mark.parametrize("rows", [65, 130, 256])
+@pytest.mark.parametrize("part,window,sinks", [(64, 0, 0), (64, 150, 4), (1024, 0, 0)])
+def test_decode_of_many_rows(nq, nkv, d, bs, rows, part, window, sinks):
+    """More rows than a wave's lanes work the runs out for at once: ragged lengths, many of them none, one far longer than the others."""
+    gen = torch.Generator().manual_seed(rows + part + nq)
+    ctx = torch.randint(0, 300, (rows,), generator=gen)
+    ctx[torch.rand(rows, generator=gen) < 0.3] = 0
+    ctx[rows - 3], ctx[0], ctx[64] = 1000, 0, 290
+    ctx = ctx.tolist()
+    nb, bt = _tables(gen, ctx, bs)
+    kc, vc = _random_cache(gen, nb, nkv, bs, d)
+    q = _queries(gen, rows, nq, nkv, d)
+    want, size = _oracle_rows(q, kc, vc, bt, ctx, nq, nkv, d, window, sinks)
+    got = _decode(get_ops("cuda"), "cuda", q, kc, vc, bt, ctx, nq, nkv, d, bs, part, window, sinks)
+    _check(got, want, size)
+    assert not got[torch.tensor(ctx) == 0].any()
+
+
+def _dense(rows, ctx, nq, nkv, bs, width, window, sinks):
+    """Whether the prompt kernel takes a call's workgroups tile by tile (else those of a tile come apart, as few rows and split keys have them)."""
+    g, tiles = nq // nkv, sum(-(-r // 128) for r in rows)
+    heads = next(h for h in (8, 4, 2, 1) if g % h == 0)
+    qr, slots = (128, 512) if heads == 1 else (256 // heads, 256)
+    wgs = tiles * (128 // qr) * (nq // heads)
+    live = min(wgs, (sum(rows) // qr + len(rows)) * (nq // heads))
+    seen = min(width * bs, window + sinks + qr + 128) if window else width * bs
+    splits = 1 if wgs > 2048 else max(1, min(slots // live, seen // 64 // 8))
+    return splits == 1 and 4 * sum(rows) > 3 * 128 * tiles
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("nq,nkv,d,bs", [(32, 2, 128, 16), (16, 2, 96, 32), (8, 1, 64, 16), (16, 4, 128, 64), (8, 4, 128, 16), (4, 2, 96, 16),
+                                         (6, 6, 128, 16), (5, 1, 64, 32), (10, 2, 96, 16)])
+@pytest.mark.parametrize("window,sinks", [(0, 0), (200, 70), (130, 0)])
+@pytest.mark.parametrize("rows,ctx", [([256, 384, 127], [256, 900, 400]), ([640], [890])])
+def test_full_prompt_steps(nq, nkv, d, bs, window, sinks, rows, ctx):
+    """Tiles full of rows, behind a cached beginning or not, for 16, 8, 4, 2, 1 and 5 queries a kv head; a NaN value and a page that is none."""
+    gen = torch.Generator().manual_seed(nq + d + len(rows))
+    nb, bt = _tables(gen, ctx, bs)
+    assert _dense(rows, ctx, nq, nkv, bs, bt.shape[1], window, sinks) and sum(-(-r // 128) for r in rows) >= 5
+    kc, vc = _random_cache(gen, nb, nkv, bs, d)
+    _spoil((kc, vc), bt, bs, d, 0, 250, nkv - 1, d // 32 - 1)
+    bt[-1, 300 // bs] = -1
+    q = _queries(gen, sum(rows) + 2, nq, nkv, d)
+    out = torch.full((sum(rows) + 2, nq * d), 3.0, device="cuda", dtype=torch.bfloat16)
+    _prompt(get_ops("cuda"), "cuda", q, kc, vc, bt, rows, ctx, nq, nkv, d, window, sinks, out=out)
+    want, size = _oracle(q, kc, vc, bt, rows, ctx, nq, nkv, 1 / math.sqrt(d), window, sinks)
+    assert want.isnan().any()
+    _check(out[:-2], want, size)
+    assert (out[-2:] == 3).all()
+
+
 @pytest.mark.gpu
 @pytest.mark.parametrize("nq,nkv,d,bs", [(32, 8, 128, 16), (16, 1, 128, 64), (7, 7, 96, 16), (14, 7, 64, 32), (28, 4, 96, 256)])
 @pytest.mark.parametrize("window,sinks", [(0, 0), (2000, 70), (700, 0)])
