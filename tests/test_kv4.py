@@ -730,6 +730,30 @@ def test_hidden_nans_stay_hidden_and_seen_ones_show(dev, d, window, sinks):
 
 
 @pytest.mark.parametrize("dev", DEVICES)
+@pytest.mark.parametrize("nq,nkv,d", [(8, 2, 64), (3, 3, 96), (16, 2, 128)])
+@pytest.mark.parametrize("value", [float("nan"), float("inf"), float("-inf")])
+def test_a_query_that_is_no_number(dev, nq, nkv, d, value):
+    """A NaN or an infinity in any 32 dims of a query makes that row of that head NaN (a score of infinity has no softmax) and no other."""
+    gen = torch.Generator().manual_seed(d)
+    bs, n = 16, 200
+    nb, bt = _tables(gen, [n], bs)
+    kc, vc = _random_cache(gen, nb, nkv, bs, d)
+    q = _queries(gen, n, nq, nkv, d)
+    spoiled = [(3 + 40 * g, g % nq, 32 * g + 7 * g) for g in range(d // 32)]
+    for row, head, dim in spoiled:
+        q[row, head * d + dim] = value
+    clean = q[:, : nq * d].float().nan_to_num(0.0, 0.0, 0.0).to(torch.bfloat16)
+    want, size = _oracle(clean, kc, vc, bt, [n], [n], nq, nkv, 1 / math.sqrt(d), 0, 0)
+    for row, head, _ in spoiled:
+        want[row, head] = float("nan")
+    _check(_prompt(get_ops(dev), dev, q, kc, vc, bt, [n], [n], nq, nkv, d, 0, 0), want, size)
+    rows = [r for r, _, _ in spoiled]
+    for part in (64, 256):
+        got = _decode(get_ops(dev), dev, q[rows], kc, vc, bt.repeat(len(rows), 1), [r + 1 for r in rows], nq, nkv, d, bs, part, 0, 0)
+        _check(got, want[rows], size[rows])
+
+
+@pytest.mark.parametrize("dev", DEVICES)
 def test_pages_outside_of_the_cache_are_not_seen(dev):
     """Block ids below 0 and behind the cache: their keys are hidden, a row without any other is zeros; a context longer than its
     table ends with the table."""
