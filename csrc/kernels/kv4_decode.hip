@@ -483,8 +483,8 @@ static void kv4_decode(const Kv4Attn& a, const int* ctx, float* tmp_out, float* 
   if (max_parts > 1) kv4_decode_merge_kernel<D><<<dim3(a.nq, B), 256, 0, s>>>(a, ctx, tmp_out, tmp_ml, B, max_parts, out16);
 }
 
-void launch_kv4_decode(const Kv4Attn& a, const int* context_lens, float* tmp_out, float* tmp_ml, int B, int part_size,
-                       int max_parts, void* out16, hipStream_t s) {
+void launch_kv4_decode(const Kv4Attn& a, const int* context_lens, float* tmp_out, float* tmp_ml, int B, int max_parts,
+                       void* out16, hipStream_t s) {
   if (B <= 0) return;
   auto* o16 = static_cast<unsigned short*>(out16);
   if (a.cache.D == 128) kv4_decode<128>(a, context_lens, tmp_out, tmp_ml, B, max_parts, o16, s);

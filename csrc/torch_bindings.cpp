@@ -375,6 +375,7 @@ void paged_decode_mx4(at::Tensor& out, const at::Tensor& q, const at::Tensor& k_
   // the kernel cuts all sequences' keys into runs by their number of chunks of 64, which it counts in 32 bits
   TORCH_CHECK(B * (block_tables.size(1) * a.cache.block_size / 64 + 1) <= INT32_MAX,
               "paged_decode: block tables of over 2^31 chunks of 64 tokens in all");
+  // the interface of the other caches: here it only says how many partitions the workspace has to have; runs are the kernel's choice
   TORCH_CHECK(part_size > 0 && part_size % 64 == 0 && part_size <= 16384, "paged_decode: partitions of a multiple of 64 tokens, at most 16384");
   for (const at::Tensor* t : {&tmp_out, &tmp_ml})
     TORCH_CHECK(t->device() == k_cache.device() && t->scalar_type() == at::kFloat && t->is_contiguous() && t->dim() == 4 &&
@@ -384,7 +385,7 @@ void paged_decode_mx4(at::Tensor& out, const at::Tensor& q, const at::Tensor& k_
   TORCH_CHECK(tmp_ml.size(2) * part_size >= block_tables.size(1) * a.cache.block_size,
               "workspace partitions must cover block_tables capacity");
   c10::hip::HIPGuardMasqueradingAsCUDA g(k_cache.device());
-  hipserve::launch_kv4_decode(a, ctx, tmp_out.data_ptr<float>(), tmp_ml.data_ptr<float>(), (int)B, (int)part_size,
+  hipserve::launch_kv4_decode(a, ctx, tmp_out.data_ptr<float>(), tmp_ml.data_ptr<float>(), (int)B,
                               (int)tmp_ml.size(2), out16_ptr(out16, out), cur_stream());
 }
 void prefill_attention_mx4(at::Tensor& out, const at::Tensor& q, const at::Tensor& k_cache, const at::Tensor& v_cache,

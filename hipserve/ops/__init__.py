@@ -260,7 +260,8 @@ class KernelOps:
 
     def paged_decode(self, out, q, k_cache, v_cache, block_tables, context_lens, tmp_out, tmp_ml,
                      nq, nkv, part_size, scale, window=0, out16=None, sinks=0):
-        """sinks: first tokens that stay visible beside the window (4-bit cache)."""
+        """sinks: first tokens that stay visible beside the window (4-bit cache, where a workspace's partitions are the most runs that a
+        row's keys are cut into: how many depends on every row of the call, and so do a row's last bits)."""
         if kv4.is_kv4(k_cache):
             self._op.paged_decode_mx4(out, q, k_cache, v_cache, block_tables, context_lens, tmp_out, tmp_ml,
                                       nq, nkv, part_size, scale, window, sinks, out16)
