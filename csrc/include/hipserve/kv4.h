@@ -63,18 +63,22 @@ HS_DEVICE unsigned kv4_widen2(unsigned w, float s) {
   return __builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, s, kByte));
 }
 
-// 8 bf16 values over scale (its exponent) as e4m3 numbers hi + lo / 16: the nearest number to each and what that leaves. The rest is taken
-// from hi as it was converted: where hi is subnormal (below 2^-6) it has fewer than four bits, and lo holds what they lack down to 2^-13.
+// 8 bf16 values over scale (its exponent) as e4m3 numbers hi + lo / 16: the upper four of their eight significant bits (cut: bf16's
+// largest values would round up out of 32 bits' range), and the rest. The rest is taken from hi as it was converted: where hi is subnormal
+// (below 2^-6) it has fewer than four bits, and lo holds what they lack down to 2^-13.
 HS_DEVICE void kv4_split8(const u16x8 v, float scale, float scale16, u32x2& hi, u32x2& lo) {
   typedef short i16x2 __attribute__((ext_vector_type(2)));
 #pragma unroll
   for (int w = 0; w < 2; ++w) {
-    float x[4];
+    float x[4], h[4];
 #pragma unroll
-    for (int j = 0; j < 4; ++j) x[j] = bf16_to_f32(v[4 * w + j]);
+    for (int j = 0; j < 4; ++j) {
+      x[j] = bf16_to_f32(v[4 * w + j]);
+      h[j] = __uint_as_float(__float_as_uint(x[j]) & 0xfff00000u);
+    }
     i16x2 hp = {0, 0}, lp = {0, 0};
-    hp = __builtin_amdgcn_cvt_scalef32_pk_fp8_f32(hp, x[0], x[1], scale, false);
-    hp = __builtin_amdgcn_cvt_scalef32_pk_fp8_f32(hp, x[2], x[3], scale, true);
+    hp = __builtin_amdgcn_cvt_scalef32_pk_fp8_f32(hp, h[0], h[1], scale, false);
+    hp = __builtin_amdgcn_cvt_scalef32_pk_fp8_f32(hp, h[2], h[3], scale, true);
     hi[w] = __builtin_bit_cast(unsigned, hp);
     const auto h0 = __builtin_amdgcn_cvt_scalef32_pk_f32_fp8(hi[w], scale, false);
     const auto h1 = __builtin_amdgcn_cvt_scalef32_pk_f32_fp8(hi[w], scale, true);

@@ -468,6 +468,31 @@ def test_small_values_of_a_query_beside_a_large_one(dev, d, dim):
         assert (off <= tol).all(), f"off by {(off / tol).max():.3f} of what the query's parts allow"
 
 
+@pytest.mark.parametrize("dev", DEVICES)
+@pytest.mark.parametrize("d", [64, 96, 128])
+@pytest.mark.parametrize("power", [127, 126, 0, -100, -111, -117])
+def test_queries_from_the_smallest_to_the_largest(dev, d, power):
+    """2^power with each of 128 mantissas against one key, 2^power alone against another, all but exact: scores m / sqrt(d) apart, an
+    output of 6 / (1 + exp(-m / sqrt(d))) whose only errors are the roundings of probability and output and a few 32-bit steps."""
+    nq, nkv, bs = 16, 1, 16
+    kc, vc = (torch.zeros(kv4.cache_shape(1, nkv, bs, d), dtype=torch.uint8) for _ in "kv")
+    k, v = kc.view(-1), vc.view(-1)
+    k[bs * d // 2:], v[bs * d // 2:] = 127 + 8 - power, 127
+    k[3 // 2] = 1 << 4                                         # token 0: 0.5 2^(8 - power) of dim 3
+    k[d // 2 + 40 // 2] = 1                                    # token 1: of dim 40
+    v[:bs * d // 2:bs] = 0x77                                  # token 0: 6, token 1: 0
+    m = torch.arange(128, dtype=torch.float64).view(8, nq)
+    q = torch.zeros(8, nq + 2 * nkv, d, dtype=torch.float64)
+    q[:, :nq, 3], q[:, :nq, 40] = (1 + m / 128) * 2.0 ** power, 2.0 ** power
+    q = q.flatten(1).to(torch.bfloat16)
+    bt = torch.zeros(8, 1, dtype=torch.int32)
+    want = (6 / (1 + torch.exp(-m / math.sqrt(d)))).view(8, nq, 1)
+    for got in (_decode(get_ops(dev), dev, q, kc, vc, bt, [2] * 8, nq, nkv, d, bs, 64, 0, 0),
+                _prompt(get_ops(dev), dev, q, kc, vc, bt, [1] * 8, [2] * 8, nq, nkv, d, 0, 0)):
+        off = (got.float().cpu().double().view(8, nq, d) - want).abs()
+        assert (off <= (2 ** -8 + 2 ** -11 + 2 ** -8) * want).all()
+
+
 def _chunks(n, window, sinks):
     """Chunks of 64 keys that a decode row of n keys takes: those of the first keys, then the window's."""
     lo = max(0, n - window) if window else 0
