@@ -572,7 +572,10 @@ int kv4_prefill_splits(const Kv4Attn& a, int seqs, int rows, int ntiles, long* f
   const long live = min(wgs, ((long)rows / QR + seqs) * (a.nq / HG));  // that have rows, at most
   const long cap = (long)a.bt_width * a.cache.block_size;
   const long seen = a.window > 0 ? min(cap, (long)a.window + a.sinks + QR + 2 * kKv4Tile) : cap;  // at most, by a workgroup
-  const long splits = live <= 0 || wgs > 2048 ? 1 : max(1l, min(slots / live, seen / kKv4Tile / kKv4LeastRun));
+  // a workgroup's part is 133 KB at most, and no call takes more than slots * 128 / QR of them (136 MB): tiles beyond those of its rows, as a
+  // padded list has them, leave room for fewer runs
+  const long most = min(slots / max(live, 1l), slots * (128 / QR) / max(wgs, 1l));
+  const long splits = live <= 0 || wgs > 2048 ? 1 : max(1l, min(most, seen / kKv4Tile / kKv4LeastRun));
   *floats = splits > 1 ? wgs * splits * NWV * 32 * (a.cache.D + 2) : 0;
   return (int)splits;
 }

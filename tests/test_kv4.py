@@ -645,6 +645,27 @@ def test_few_rows_over_long_contexts(nq, nkv, d, bs, window, sinks, rows, ctx):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("nq,nkv,d", [(16, 2, 128), (8, 2, 64), (3, 3, 96)])
+def test_a_padded_list_of_tiles(nq, nkv, d):
+    """Tiles of no sequence behind those of the rows: skipped, and no workspace is taken for their parts (4 GB of them with 16 queries)."""
+    gen = torch.Generator().manual_seed(nq)
+    bs, rows, ctx = 16, [3], [8192]
+    nb, bt = _tables(gen, ctx, bs)
+    kc, vc = (c.cuda() for c in _random_cache(gen, nb, nkv, bs, d))
+    q = _queries(gen, 3, nq, nkv, d).cuda()
+    want, size = _oracle(q, kc, vc, bt, rows, ctx, nq, nkv, 0.1, 0, 0)
+    ints = lambda *x: torch.tensor(x, device="cuda", dtype=torch.int32)  # noqa: E731
+    tiles = torch.cat((_tiles(rows), torch.tensor([[-1, 0]], dtype=torch.int32).expand(255, -1))).cuda()
+    out, bt, cu, ctx = torch.empty(3, nq * d, device="cuda", dtype=torch.bfloat16), bt.cuda(), ints(0, 3), ints(8192)
+    torch.cuda.synchronize()
+    torch.cuda.reset_peak_memory_stats()
+    held = torch.cuda.memory_allocated()
+    get_ops("cuda").prefill_attention(out, q, kc, vc, bt, cu, ctx, tiles, nq, nkv, 0.1)
+    assert torch.cuda.max_memory_allocated() - held < 140 << 20
+    _check(out, want, size)
+
+
+@pytest.mark.gpu
 def test_two_streams_at_once():
     """Steps of two sequences on streams of their own, at the same time, give what each gives alone."""
     ops, nq, nkv, d, bs = get_ops("cuda"), 16, 2, 128, 16
