@@ -23,8 +23,8 @@
 // Hidden keys have score -inf whatever they hold. A value's NaN (scale byte 255) must reach the rows that see it alone, and 0 * NaN is
 // not 0: it is staged as a finite number and put into the accumulators of the rows that see it, in a branch that no other tile takes.
 //
-// 32 / 8 heads of 128 dims: 8192 rows 543 us (1.01 PFLOP/s), 4096 rows at 16384 825 us (1.16), a window of 4096 there 269 us; the 8-bit
-// part of the products is twice the bf16 part's operations, so this is what a bf16 cache's kernel does (530, 876, 276 us) at 17 / 64 of its bytes.
+// 32 / 8 heads of 128 dims: 8192 rows 542 - 589 us (0.93 - 1.01 PFLOP/s), 4096 rows at 16384 846 us (1.14), a window of 4096 there 266 us; the 8-bit
+// part of the products is twice the bf16 part's operations, so this is what a bf16 cache's kernel does (530 - 584, 878, 274 us) at 17 / 64 of its bytes.
 #include <atomic>
 
 #include "hipserve/kv4.h"
