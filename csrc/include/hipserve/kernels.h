@@ -86,7 +86,7 @@ struct Kv4Attn {
   float scale;
   int window, sinks;  // window > 0: keys within window - 1 positions before the query, and the first `sinks` ones
 };
-// tmp_out, tmp_ml [B, nq, max_parts, D | 2]: a row's keys are cut into max_parts runs at most (1: no run is merged, and neither is read)
+// tmp_out, tmp_ml [B, nq, max_parts, D | 2]: a row's keys are cut into max_parts runs at most (1: neither is used)
 void launch_kv4_decode(const Kv4Attn& a, const int* context_lens, float* tmp_out, float* tmp_ml, int B, int max_parts, void* out16,
                        hipStream_t s);
 // into how many runs of keys a call's rows are split at most, and the fp32 workspace that takes (0: none)
